@@ -304,7 +304,7 @@ def run(state):
         if own:
             cache, batch = _handles(state)
             cache.append(batch, state["k"], state["v"])
-            k, v = cache.read(batch, dtype=state["k"].dtype)
+            k, v = cache.read(batch, state["k"].shape[0], dtype=state["k"].dtype)
             return {"k": k, "v": v}
         return _plain_append(state)
     if own:
