@@ -459,6 +459,101 @@ int nexus_cuda_attention_noalloc(nexus_cuda_backend *b, const float *q_dev, cons
                                  size_t num_kv_heads, size_t head_dim, size_t seq_len, float scale);
 
 /* ======================================================================== */
+/* Quantised paged KV cache (no counterpart in the reference, whose          */
+/* KvCacheBuffer::Quantized, src/engine/mod.rs:187-313, packs one token over */
+/* all heads and serves one token of one sequence at a time)                 */
+/* ======================================================================== */
+/* For callers that run their own layers: the cache of one layer in buffers
+ * of the caller, written and attended for a ragged batch of sequences in one
+ * call each.  Keys and values are held in 8 or 4 bits, one group of head_dim
+ * elements per (token, KV head):
+ *   8 bits: scale = max|x| / 127,         value = scale * (code - 128)
+ *   4 bits: scale = (max x - min x) / 15, zero = min x + 8 * scale,
+ *           value = zero + scale * (code - 8)
+ * (scale and zero rounded to f32, code the nearest integer, ties to even).  A
+ * group that holds a NaN or an infinity, or spans more than f32, reads back
+ * as NaN. */
+typedef struct {
+    uint32_t kv_heads;
+    uint32_t head_dim;      /* 32, 64 or 128 */
+    uint32_t page_tokens;   /* tokens of a page, a power of two in [16, 4096] */
+    uint32_t num_pages;     /* pages of the pool */
+    uint32_t bits_k, bits_v; /* 8 or 4 each */
+    /* device, 16-byte aligned.  codes: [num_pages][kv_heads][page_tokens]
+     * [head_dim * bits / 8] bytes, LSB first; scales: [num_pages][kv_heads]
+     * [page_tokens] f32 (8 bits), or (scale, zero) pairs (4 bits) */
+    void *k_codes, *v_codes;
+    float *k_scales, *v_scales;
+} nexus_kv_cache;
+
+/* A ragged batch.  Sequence b brings the rows [q_start[b], q_start[b + 1]) of
+ * the row tensors, the last of its kv_len[b] tokens (kv_len counts them): row
+ * q_start[b] + i is token kv_len[b] - n + i of n.  Rows whose token number
+ * would be negative are padding: append skips them, read and attention give
+ * zeros.  Rows outside every sequence are left as they were.  Token t lives in
+ * page page_table[b * table_stride + t / page_tokens]; entries of pages that
+ * hold no token a call reads or writes are not looked at, and a page may be
+ * listed for several sequences that read it, but the slot a call writes must
+ * be one sequence's.  q_start, kv_len and page_table are device arrays, so a
+ * captured call follows their contents; max_q and max_kv are host bounds of
+ * what they will hold. */
+typedef struct {
+    uint32_t n_seqs;
+    uint32_t max_q;         /* most new tokens of any sequence */
+    uint32_t max_kv;        /* longest kv_len */
+    uint32_t table_stride;  /* page table entries per sequence */
+    const uint32_t *q_start, *kv_len, *page_table; /* device */
+    void *stream;           /* cudaStream_t the call runs on, with NEXUS_KV_CALLER_STREAM */
+    uint32_t flags;
+} nexus_kv_batch;
+#define NEXUS_KV_CALLER_STREAM 0x1u /* run on batch.stream (NULL: the legacy default stream) instead of the
+                                       backend's stream */
+
+/* Rows [rows][heads][head_dim] on the device: f32, f16 or bf16, elements of a
+ * head adjacent, 16-byte aligned data and strides (strides in elements). */
+typedef struct {
+    void *data;
+    int format;             /* NEXUS_FMT_F32, NEXUS_FMT_F16 or NEXUS_FMT_BF16 */
+    uint32_t heads;
+    size_t rows;
+    size_t row_stride, head_stride;
+} nexus_kv_rows;
+
+/* All calls below are asynchronous on the call's stream, keep nothing between
+ * calls and may be captured into a CUDA graph.  Arguments are checked before
+ * anything is launched; what only the device can see (a page id beyond the
+ * pool, q_start out of order, lengths beyond max_q, max_kv or the page table)
+ * makes the kernels skip the sequence or page and is reported by
+ * nexus_cuda_kv_status. */
+
+/* Quantises the batch's rows of k and v into their page slots. */
+int nexus_cuda_kv_append(nexus_cuda_backend *b, const nexus_kv_cache *cache, const nexus_kv_batch *batch,
+                         const nexus_kv_rows *k, const nexus_kv_rows *v);
+/* Writes the values that the cache holds for the batch's rows (k or v may be NULL). */
+int nexus_cuda_kv_read(nexus_cuda_backend *b, const nexus_kv_cache *cache, const nexus_kv_batch *batch,
+                       const nexus_kv_rows *k, const nexus_kv_rows *v);
+/* Causal GQA attention of the batch's query rows over the cache, which holds
+ * their own tokens already: the query at position i sees key j when j <= i and
+ * (window == 0 or j > i - window or j < sinks).  Query head q uses KV head
+ * q / (q heads / kv heads); at most 128 query heads per KV head.  scale 0
+ * means 1/sqrt(head_dim).  out has q's format and heads.  The workspace
+ * (device, 16-byte aligned, contents free before and after) holds at least
+ * nexus_cuda_kv_attention_workspace bytes and belongs to this call until it
+ * has run: calls that may overlap need one each. */
+int nexus_cuda_kv_attention(nexus_cuda_backend *b, const nexus_kv_cache *cache, const nexus_kv_batch *batch,
+                            const nexus_kv_rows *q, const nexus_kv_rows *out, float scale, uint32_t window,
+                            uint32_t sinks, void *workspace, size_t workspace_bytes);
+/* Workspace bytes of that call (0: none needed); depends on the sizes, formats
+ * and bounds only.  Host arithmetic, no device. */
+int nexus_cuda_kv_attention_workspace(const nexus_kv_cache *cache, const nexus_kv_batch *batch,
+                                      const nexus_kv_rows *q, uint32_t window, uint32_t sinks, size_t *bytes);
+/* Waits for the stream (NULL with flags 0: the backend's) and reports, then
+ * clears, what this backend's KV calls found wrong on the device:
+ * NEXUS_E_INVALID with a message, NEXUS_E_TIMEOUT for a wait that gave up.
+ * Not for use during stream capture. */
+int nexus_cuda_kv_status(nexus_cuda_backend *b, void *stream, uint32_t flags);
+
+/* ======================================================================== */
 /* Host utilities (the reference's converter and quantizers)                 */
 /* ======================================================================== */
 

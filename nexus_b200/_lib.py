@@ -103,6 +103,25 @@ class SynthConfig(C.Structure):
                 ("threads", C.c_int), ("repeat_chunks", C.c_uint32)]
 
 
+class KvCache(C.Structure):
+    _fields_ = [("kv_heads", C.c_uint32), ("head_dim", C.c_uint32), ("page_tokens", C.c_uint32),
+                ("num_pages", C.c_uint32), ("bits_k", C.c_uint32), ("bits_v", C.c_uint32),
+                ("k_codes", C.c_void_p), ("v_codes", C.c_void_p), ("k_scales", C.c_void_p), ("v_scales", C.c_void_p)]
+
+
+class KvBatch(C.Structure):
+    _fields_ = [("n_seqs", C.c_uint32), ("max_q", C.c_uint32), ("max_kv", C.c_uint32), ("table_stride", C.c_uint32),
+                ("q_start", C.c_void_p), ("kv_len", C.c_void_p), ("page_table", C.c_void_p),
+                ("stream", C.c_void_p), ("flags", C.c_uint32)]
+
+
+class KvRows(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("format", C.c_int), ("heads", C.c_uint32), ("rows", C.c_size_t),
+                ("row_stride", C.c_size_t), ("head_stride", C.c_size_t)]
+
+
+KV_CALLER_STREAM = 0x1
+
 P = C.c_void_p
 # (name, restype, argtypes) of every symbol declared in include/nexus_cuda.h
 class TpSlice(C.Structure):
@@ -168,6 +187,15 @@ SIGNATURES = [
                                             C.c_int, C.POINTER(C.c_int)]),
     ("nexus_cuda_attention_noalloc", C.c_int, [P, P, P, P, P, C.c_size_t, C.c_size_t, C.c_size_t, C.c_size_t,
                                                C.c_float]),
+    ("nexus_cuda_kv_append", C.c_int, [P, C.POINTER(KvCache), C.POINTER(KvBatch), C.POINTER(KvRows),
+                                       C.POINTER(KvRows)]),
+    ("nexus_cuda_kv_read", C.c_int, [P, C.POINTER(KvCache), C.POINTER(KvBatch), C.POINTER(KvRows),
+                                     C.POINTER(KvRows)]),
+    ("nexus_cuda_kv_attention", C.c_int, [P, C.POINTER(KvCache), C.POINTER(KvBatch), C.POINTER(KvRows),
+                                          C.POINTER(KvRows), C.c_float, C.c_uint32, C.c_uint32, P, C.c_size_t]),
+    ("nexus_cuda_kv_attention_workspace", C.c_int, [C.POINTER(KvCache), C.POINTER(KvBatch), C.POINTER(KvRows),
+                                                    C.c_uint32, C.c_uint32, C.POINTER(C.c_size_t)]),
+    ("nexus_cuda_kv_status", C.c_int, [P, P, C.c_uint32]),
     ("nexus_quantize_host", C.c_size_t, [C.c_int, P, C.c_size_t, P]),
     ("nexus_format_bytes", C.c_size_t, [C.c_int, C.c_size_t]),
     ("nexus_synth_model_write", C.c_int, [C.c_char_p, C.POINTER(SynthConfig)]),

@@ -34,11 +34,17 @@ UNITS = {
     "kernels_attn.cu": [],
     "kernels_attn_pk.cu": [],
     "kernels_attn_prefill.cu": [],
+    "kernels_kv.cu": [],
+    "kernels_kv_few_d32.cu": [],
+    "kernels_kv_few_d64.cu": [],
+    "kernels_kv_few_d128.cu": [],
+    "kernels_kv_merge.cu": [],
     "kernels_step.cu": [],
     "kernels_peer.cu": [],
     "kernels_misc.cu": [],
     "engine.cu": [],
     "noalloc.cu": [],
+    "kvcache.cu": [],
 }
 CXX_UNITS = ["host.cpp", "scheduler.cpp"]
 

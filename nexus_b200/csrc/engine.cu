@@ -48,6 +48,9 @@ struct nexus_cuda_backend {
     bool destroy_pending = false;
     // set by a kernel whose bounded wait gave up (op-level calls)
     int *dev_err = nullptr;
+    // what the paged KV cache calls found wrong on the device (kvcache.cu):
+    // [0] KvFault bits, [1] the bits nexus_cuda_kv_status takes
+    unsigned *kv_fault = nullptr;
     // tensor parallelism (nexus_cuda_tp_init)
     int tp_rank = 0, tp_world = 1;
     ncclComm_t comm = nullptr;
@@ -128,6 +131,7 @@ static void backend_free_now(nexus_cuda_backend *b) {
         cudaStreamDestroy(b->stream);
     }
     if (b->dev_err) cudaFree(b->dev_err);
+    if (b->kv_fault) cudaFree(b->kv_fault);
     peer_release(b);
     if (b->comm) {
         if (NcclApi *api = nccl_api(nullptr)) api->comm_destroy(b->comm);
@@ -310,7 +314,17 @@ int nexus_backend_stream_device(nexus_cuda_backend *b, cudaStream_t *stream, int
     return NEXUS_OK;
 }
 
-int nexus_backend_fail(nexus_cuda_backend *b, int code, const char *msg) { return set_err(b, code, msg); }
+unsigned *nexus_backend_kv_fault(nexus_cuda_backend *b) { return b->kv_fault; }
+
+int nexus_backend_fail(nexus_cuda_backend *b, int code, const char *msg) {
+    try {
+        static std::mutex mu;  // calls from several threads may fail at once
+        std::lock_guard<std::mutex> lk(mu);
+        return set_err(b, code, msg);
+    } catch (...) {  // no memory for the message: the status stands alone
+        return code;
+    }
+}
 
 extern "C" void nexus_cuda_config_default(nexus_cuda_config *cfg) {
     memset(cfg, 0, sizeof(*cfg));
@@ -378,7 +392,12 @@ extern "C" int nexus_cuda_backend_create(const nexus_cuda_config *cfg, nexus_cud
     if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&b->stream, cudaStreamNonBlocking);
     if (e == cudaSuccess) e = cudaMalloc((void **)&b->dev_err, sizeof(int));
     if (e == cudaSuccess) e = cudaMemset(b->dev_err, 0, sizeof(int));
+    if (e == cudaSuccess) e = cudaMalloc((void **)&b->kv_fault, 2 * sizeof(unsigned));
+    if (e == cudaSuccess) e = cudaMemset(b->kv_fault, 0, 2 * sizeof(unsigned));
+    if (e == cudaSuccess) e = cudaStreamSynchronize(cudaStreamLegacy);  // other streams may use them next
     if (e != cudaSuccess) {
+        if (b->dev_err) cudaFree(b->dev_err);
+        if (b->kv_fault) cudaFree(b->kv_fault);
         if (b->stream) cudaStreamDestroy(b->stream);
         delete b;
         return set_err(nullptr, NEXUS_E_CUDA, std::string("backend init: ") + cudaGetErrorString(e));

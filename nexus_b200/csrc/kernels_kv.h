@@ -1,0 +1,59 @@
+// kernels_kv.h -- launch interfaces of the quantised paged KV cache operators.
+#pragma once
+#include <cuda_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#include "kv_plan.h"
+
+namespace nx {
+
+// Caller-owned cache of one layer: codes [page][kv head][slot][D * bits / 8],
+// scales [page][kv head][slot][1 (8 bits) or 2 (4 bits)].  Index 0: keys, 1: values.
+struct KvCacheView {
+    uint8_t *codes[2];
+    float *scales[2];
+    int bits[2];
+    uint32_t hkv, num_pages, shift;
+    int head_dim;
+};
+
+// Rows [row][head][head_dim] with strides in elements; fmt is a NEXUS_FMT_* id.
+struct KvRows {
+    void *data;
+    int fmt;
+    size_t row_stride, head_stride;
+};
+
+struct KvCopyParams {
+    KvCacheView cache;
+    KvBatchView batch;
+    KvRows rows[2];   // keys, values; data == nullptr: side not wanted (read)
+    unsigned *fault;
+};
+cudaError_t launch_kv_append(const KvCopyParams &p, cudaStream_t st);
+cudaError_t launch_kv_read(const KvCopyParams &p, cudaStream_t st);
+
+struct KvAttnParams {
+    KvCacheView cache;
+    KvBatchView batch;
+    KvRows q, out;
+    int hq, group;
+    float scale_log2;          // score scale * log2(e)
+    uint32_t window, sinks;
+    unsigned *fault;
+    // split over the context
+    uint32_t nsplit, tiles_per_split;
+    float *part;               // records of unfinished softmaxes (nsplit > 1)
+    uint32_t rows_limit;       // sequences of at most so many (token, head) rows per KV head
+    uint32_t tile_rows, row_tiles;  // rows of a tile (8 or 16), tiles a sequence may have
+};
+
+constexpr uint32_t kKvFewTile = 16;      // tokens of one warp's tile
+constexpr uint32_t kKvFewWarps = 4;
+constexpr uint32_t kKvSms = 148;
+
+cudaError_t launch_kv_attn_few(const KvAttnParams &p, cudaStream_t st);
+cudaError_t launch_kv_merge_few(const KvAttnParams &p, cudaStream_t st);
+
+}  // namespace nx

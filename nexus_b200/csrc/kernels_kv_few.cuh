@@ -1,0 +1,576 @@
+// kernels_kv_few.cuh -- attention of a few query rows (a decode token, a short
+// draft window) over the quantised paged KV cache.
+//
+// For one (sequence, KV head) the rows are the new tokens x the G query heads
+// of the group (row r: token r / G, head r % G of the group), in tiles of 8 or 16.  With key j = zk_j + sk_j * kc_j (kc integer codes
+// around zero, zk = 0 for 8 bits) and likewise values:
+//   x_rj = c_r * (sk_j * (q_r . kc_j) + zk_j * sum(q_r)),  p = 2^(x - m_r)
+//   o_r  = [ 2^(R_r) sum_j (p sv_j 2^(m_r - R_r)) vc_j + sum_j p zv_j ] / sum_j p,  R_r = B_r - 14
+// so the two products run on exact small integers in f16 and everything that
+// is not an integer stays in f32.  The rounded factors are q (22 bits as f16
+// hi + lo for f32 queries, 11 bits otherwise: bf16 and f16 are exact) and the
+// weight p sv 2^(m - R) (f16; hi + lo for f32 queries).  m and B are whole
+// numbers at or above the largest x and x + log2(sv) so far: every rescaling
+// is by an exact power of two, and the weights lie below 2^14 with the largest
+// near it, whatever the scale of the values: f16 keeps its 11 bits down to
+// 2^-28 of the largest.
+//
+// Bound: HBM, the visible codes and scales once (264 bytes a token and head at
+// D = 128 and 8 bits, 144 at 4).  Layout:
+//  - S^T = K Q^T and O^T = V^T P^T on mma.sync.m16n8k16 (M = 16 tokens or 16
+//    dims, N = 8 rows): the rows of a decode step fill half of one N = 8 tile,
+//    where the 128-row tcgen05 tile would be empty but for 4 of 128, and both
+//    operands are unpacked in registers, which tcgen05 could not read.
+//  - A warp owns 16-token tiles (one page holds a tile whole); their codes and
+//    scales come by cp.async into a ring of four slots of its own, so three
+//    tiles a warp are in flight and no barrier is in the loop.
+//  - The context is split over CTAs; kv_merge_few joins the parts in order.
+#pragma once
+#include "kv_math.cuh"
+
+namespace nx {
+namespace kvf {
+
+constexpr int kWarps = kKvFewWarps;
+constexpr int kStages = 4;
+constexpr float kWeightUp = 14.0f;  // weights are kept below 2^14
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+__device__ __forceinline__ uint32_t f16x2(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ float2 f16x2_back(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2 *>(&v)); }
+__device__ __forceinline__ float lg2(float x) {
+    float y;
+    asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// 2^(a - b) exactly, for whole a and b, either possibly -inf (0 then); the
+// exponent is kept within f32's normal range
+__device__ __forceinline__ float pow2_diff(float a, float b) {
+    if (a == -INFINITY || b == -INFINITY) return 0.0f;
+    return __int_as_float((127 + (int)fminf(126.0f, fmaxf(-126.0f, a - b))) << 23);
+}
+
+template <int D, int BK, int BV>
+struct Tile {
+    static constexpr int RK = D * BK / 8, RV = D * BV / 8;       // code bytes of a token
+    static constexpr int K = 16 * RK, V = 16 * RV;               // code bytes of a tile
+    static constexpr int KS = BK == 8 ? 64 : 128, VS = BV == 8 ? 64 : 128;
+    static constexpr int BYTES = K + V + KS + VS;
+    static constexpr int SMEM = kWarps * kStages * BYTES;
+};
+// 16-byte chunks of a 128-byte row are stored XORed with the row, so that the
+// fragment loads of a quarter warp fall into different banks
+template <int RB>
+__device__ __forceinline__ int k_swz(int row) {
+    return RB == 128 ? 4 * (row & 1) : 0;
+}
+template <int RB>
+__device__ __forceinline__ int v_swz(int row) {
+    return RB == 128 ? 2 * ((row >> 1) & 3) : RB == 64 ? (row >> 1) & 3 : 0;
+}
+
+template <int N>
+__device__ __forceinline__ void lds_words(const uint8_t *p, uint32_t (&w)[N], int at) {
+    if constexpr (N % 4 == 0) {
+        const uint4 v = *reinterpret_cast<const uint4 *>(p);
+        w[at] = v.x;
+        w[at + 1] = v.y;
+        w[at + 2] = v.z;
+        w[at + 3] = v.w;
+    } else if constexpr (N == 2) {
+        const uint2 v = *reinterpret_cast<const uint2 *>(p);
+        w[0] = v.x;
+        w[1] = v.y;
+    } else {
+        w[0] = *reinterpret_cast<const uint32_t *>(p);
+    }
+}
+
+// Record of row r of a (sequence, KV head) pair and split s: D floats o, then m, l.
+__host__ __device__ inline size_t few_record(uint32_t pair, uint32_t rows, uint32_t r, uint32_t nsplit, uint32_t s) {
+    return ((size_t)pair * rows + r) * nsplit + s;
+}
+
+template <int D, int BK, int BV, int NR, bool SPLIT>
+__global__ void __launch_bounds__(kWarps * 32, (NR == 1 && !SPLIT) ? 3 : 2) k_kv_attn_few(KvAttnParams p) {
+    using T = Tile<D, BK, BV>;
+    constexpr int KW = D * BK / 128;       // 32-bit words of a key row per thread
+    constexpr int UNITS = D / 32;          // units of eight consecutive elements of a row per thread
+    constexpr int KSTEPS = D / 16;
+    constexpr int MT = D / 16;             // 16-dim tiles of the output
+    constexpr int NS = SPLIT ? 2 : 1;
+    extern __shared__ __align__(128) uint8_t smem[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    constexpr uint32_t R = 8 * NR;
+    const uint32_t split = blockIdx.x % p.nsplit, rt = blockIdx.x / p.nsplit, h = blockIdx.y, b = blockIdx.z;
+    unsigned fault = 0;
+    const KvSeqView seq = kv_load_seq(p.batch, b, p.cache.shift, &fault);
+    if (fault) {
+        if (threadIdx.x == 0) kv_report(p.fault, fault);
+        return;
+    }
+    const uint32_t G = (uint32_t)p.group;
+    const KvRowTile rows = kv_row_tile(seq, G, rt, R, p.rows_limit);
+    if (rows.n == 0) return;
+    const int pos0 = (int)seq.kv - (int)seq.nq;
+    const KvRange range = kv_range(rows.first, rows.last, p.window, p.sinks);
+    const KvTiles tiles = kv_tiles(range, kKvFewTile);
+    const uint32_t t_begin = split * p.tiles_per_split;
+    const uint32_t t_end = min(tiles.total, t_begin + p.tiles_per_split);
+    if (p.nsplit > 1 && t_begin >= t_end) return;  // the merge knows how many parts there are
+
+    // ---- copies: lane L of a batch of 32 tiles holds the page of tile L ----
+    const uint32_t n_mine = t_begin + warp < t_end ? (t_end - t_begin - warp + kWarps - 1) / kWarps : 0;
+    const uint32_t *table = p.batch.table + (size_t)b * p.batch.stride;
+    auto tile_token = [&](uint32_t k) { return kv_tile_at(tiles, t_begin + warp + k * kWarps) * kKvFewTile; };
+    auto load_page = [&](uint32_t k) -> uint32_t {
+        if (k >= n_mine) return 0u;
+        return __ldg(table + (tile_token(k) >> p.cache.shift));
+    };
+    uint32_t page_cur = load_page(lane), page_next = load_page(32 + lane);
+    uint8_t *ring = smem + warp * kStages * T::BYTES;
+    const uint32_t ring_s = smem_u32(ring);
+    unsigned bad = 0;  // bit k & 31: tile k has no valid page
+    auto issue = [&](uint32_t k) {
+        if (k < n_mine) {
+            if ((k & 31u) == 0 && k > 0) {
+                page_cur = page_next;
+                page_next = load_page(k + 32 + lane);
+            }
+            const uint32_t page = __shfl_sync(0xffffffffu, page_cur, k & 31u);
+            if (page < p.cache.num_pages) {
+                bad &= ~(1u << (k & 31u));
+                const size_t slot = (((size_t)page * p.cache.hkv + h) << p.cache.shift) +
+                                    (tile_token(k) & ((1u << p.cache.shift) - 1u));
+                const uint32_t dst = ring_s + (k % kStages) * T::BYTES;
+                const uint8_t *ks = p.cache.codes[0] + slot * T::RK, *vs = p.cache.codes[1] + slot * T::RV;
+#pragma unroll
+                for (int i = 0; i < (T::K / 16 + 31) / 32; i++) {
+                    const int ch = i * 32 + lane, row = ch / (T::RK / 16), col = ch % (T::RK / 16);
+                    if (T::K / 16 >= 32 || ch < T::K / 16)
+                        cp_async16(dst + row * T::RK + ((col ^ k_swz<T::RK>(row)) * 16), ks + ch * 16);
+                }
+#pragma unroll
+                for (int i = 0; i < (T::V / 16 + 31) / 32; i++) {
+                    const int ch = i * 32 + lane, row = ch / (T::RV / 16), col = ch % (T::RV / 16);
+                    if (T::V / 16 >= 32 || ch < T::V / 16)
+                        cp_async16(dst + T::K + row * T::RV + ((col ^ v_swz<T::RV>(row)) * 16), vs + ch * 16);
+                }
+                if (lane < T::KS / 16)
+                    cp_async16(dst + T::K + T::V + lane * 16,
+                               reinterpret_cast<const uint8_t *>(p.cache.scales[0]) + slot * (T::KS / 16) + lane * 16);
+                if (lane >= 16 && lane < 16 + T::VS / 16)
+                    cp_async16(dst + T::K + T::V + T::KS + (lane - 16) * 16,
+                               reinterpret_cast<const uint8_t *>(p.cache.scales[1]) + slot * (T::VS / 16) +
+                                   (lane - 16) * 16);
+            } else {
+                bad |= 1u << (k & 31u);
+                fault = KV_FAULT_PAGE;
+            }
+        }
+        cp_commit();
+    };
+#pragma unroll
+    for (int k = 0; k < kStages - 1; k++) issue(k);
+
+    // ---- queries: row g (+ 8) as the B operand, in the order of the code words ----
+    uint32_t qf[NR][NS][KSTEPS][2];
+    float x_scale[NR][2], x_sum[NR][2];  // of this thread's columns, rows 2c and 2c + 1
+    int x_pos[NR][2];
+#pragma unroll
+    for (int nr = 0; nr < NR; nr++) {
+        const uint32_t r = rows.r0 + 8 * nr + g, tok = r / G, head = h * G + r % G;
+        const bool used = (uint32_t)(8 * nr + g) < rows.n;
+        float q[UNITS][8];
+        float amax = 0.0f;
+#pragma unroll
+        for (int u = 0; u < UNITS; u++) {
+            // first element of the unit: 8-bit rows come in 16-byte chunks c and c + 4
+            // (two units each; 8 bytes at D = 32), 4-bit rows in chunks of up to 16 bytes
+            int e;
+            if constexpr (BK == 8) e = D == 32 ? 8 * c : (u >> 1) * 64 + c * 16 + (u & 1) * 8;
+            else e = c * (D / 4) + 8 * u;
+            if (used) {
+                load8(p.q.data, (size_t)(seq.q0 + tok) * p.q.row_stride + head * p.q.head_stride + e, p.q.fmt, q[u]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++) q[u][i] = 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++) amax = fmaxf(amax, fabsf(q[u][i]));
+        }
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+        const float sc = row_scale(amax);
+        float sum = 0.0f;
+#pragma unroll
+        for (int u = 0; u < UNITS; u++) {
+            // element pairs of a k step: (0,1)(2,3) then (4,5)(6,7) of 8-bit words,
+            // (0,4)(1,5) then (2,6)(3,7) of a 4-bit word
+            constexpr int o8[8] = {0, 1, 2, 3, 4, 5, 6, 7}, o4[8] = {0, 4, 1, 5, 2, 6, 3, 7};
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float v0 = q[u][BK == 8 ? o8[2 * i] : o4[2 * i]] * sc;
+                const float v1 = q[u][BK == 8 ? o8[2 * i + 1] : o4[2 * i + 1]] * sc;
+                const uint32_t hi = f16x2(v0, v1);
+                const float2 back = f16x2_back(hi);
+                qf[nr][0][2 * u + (i >> 1)][i & 1] = hi;
+                sum += back.x + back.y;
+                if constexpr (SPLIT) {
+                    const uint32_t lo = f16x2(v0 - back.x, v1 - back.y);
+                    const float2 lb = f16x2_back(lo);
+                    qf[nr][NS - 1][2 * u + (i >> 1)][i & 1] = lo;
+                    sum += lb.x + lb.y;
+                }
+            }
+        }
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        const float xs = p.scale_log2 / sc;
+        const int pos = used ? pos0 + (int)tok : -1;
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            x_scale[nr][e] = __shfl_sync(0xffffffffu, xs, (2 * c + e) * 4);
+            x_sum[nr][e] = __shfl_sync(0xffffffffu, sum, (2 * c + e) * 4);
+            x_pos[nr][e] = __shfl_sync(0xffffffffu, pos, (2 * c + e) * 4);
+        }
+    }
+
+    float o[NR][MT][4], m[NR][2], big[NR][2], fac[NR][2], l[NR][2], z[NR][2];
+#pragma unroll
+    for (int nr = 0; nr < NR; nr++) {
+#pragma unroll
+        for (int j = 0; j < MT; j++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) o[nr][j][i] = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            m[nr][e] = big[nr][e] = -INFINITY;
+            fac[nr][e] = l[nr][e] = z[nr][e] = 0.0f;
+        }
+    }
+
+    for (uint32_t k = 0; k < n_mine; k++) {
+        cp_wait<kStages - 2>();
+        __syncwarp();
+        const uint8_t *st = ring + (k % kStages) * T::BYTES;
+        const int j0 = (int)tile_token(k);
+        const bool skip = (bad >> (k & 31u)) & 1u;
+        if (!skip) {
+            // ---- S^T = K Q^T ----
+            uint32_t kw[2][KW];
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                const int row = g + 8 * t;
+                const uint8_t *kr = st + row * T::RK;
+                if constexpr (T::RK == 128) {
+                    lds_words<KW>(kr + ((c ^ k_swz<128>(row)) * 16), kw[t], 0);
+                    lds_words<KW>(kr + (((c + 4) ^ k_swz<128>(row)) * 16), kw[t], 4);
+                } else {
+                    lds_words<KW>(kr + c * (T::RK / 4), kw[t], 0);
+                }
+            }
+            float s[NR][4];
+#pragma unroll
+            for (int nr = 0; nr < NR; nr++) s[nr][0] = s[nr][1] = s[nr][2] = s[nr][3] = 0.0f;
+#pragma unroll
+            for (int ks = 0; ks < KSTEPS; ks += BK == 8 ? 1 : 2) {
+                if constexpr (BK == 8) {
+                    uint32_t a[4];
+                    unpack_u8(kw[0][ks], a[0], a[2]);
+                    unpack_u8(kw[1][ks], a[1], a[3]);
+#pragma unroll
+                    for (int nr = 0; nr < NR; nr++)
+#pragma unroll
+                        for (int n = 0; n < NS; n++) mma16816(s[nr], a, qf[nr][n][ks]);
+                } else {
+                    uint32_t u0[4], u1[4];
+                    unpack_u4(kw[0][ks >> 1], u0);
+                    unpack_u4(kw[1][ks >> 1], u1);
+#pragma unroll
+                    for (int half = 0; half < 2; half++) {
+                        const uint32_t a[4] = {u0[2 * half], u1[2 * half], u0[2 * half + 1], u1[2 * half + 1]};
+#pragma unroll
+                        for (int nr = 0; nr < NR; nr++)
+#pragma unroll
+                            for (int n = 0; n < NS; n++) mma16816(s[nr], a, qf[nr][n][ks + half]);
+                    }
+                }
+            }
+            // ---- scales of tokens j0 + g and j0 + g + 8 ----
+            float sk[2], zk[2], sv[2], zv[2], lv[2];
+            const float *kscale = reinterpret_cast<const float *>(st + T::K + T::V);
+            const float *vscale = reinterpret_cast<const float *>(st + T::K + T::V + T::KS);
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                const int i = g + 8 * t;
+                sk[t] = BK == 8 ? kscale[i] : kscale[2 * i];
+                zk[t] = BK == 8 ? 0.0f : kscale[2 * i + 1];
+                sv[t] = BV == 8 ? vscale[i] : vscale[2 * i];
+                zv[t] = BV == 8 ? 0.0f : vscale[2 * i + 1];
+                lv[t] = lg2(sv[t]);
+            }
+            // every token of the tile seen by every row?
+            const bool whole = j0 + (int)kKvFewTile - 1 <= rows.first &&
+                               (p.window == 0 || j0 > rows.last - (int)p.window ||
+                                j0 + (int)kKvFewTile <= (int)p.sinks);
+            float x[NR][4];  // [token half t][column e] at 2 t + e
+            bool grow = false;
+#pragma unroll
+            for (int nr = 0; nr < NR; nr++)
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        float v = s[nr][2 * t + e] * sk[t];
+                        if constexpr (BK == 4) v = fmaf(zk[t], x_sum[nr][e], v);
+                        v *= x_scale[nr][e];
+                        if (!whole && !kv_visible(j0 + g + 8 * t, x_pos[nr][e], (int)p.window, (int)p.sinks))
+                            v = -INFINITY;
+                        x[nr][2 * t + e] = v;
+                        grow |= v > m[nr][e] || v + lv[t] > big[nr][e];
+                    }
+            if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+                for (int nr = 0; nr < NR; nr++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        float mx = fmaxf(x[nr][e], x[nr][2 + e]);
+                        float my = fmaxf(x[nr][e] + lv[0], x[nr][2 + e] + lv[1]);
+#pragma unroll
+                        for (int w = 4; w < 32; w <<= 1) {
+                            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
+                            my = fmaxf(my, __shfl_xor_sync(0xffffffffu, my, w));
+                        }
+                        const float m1 = fmaxf(m[nr][e], ceilf(mx)), b1 = fmaxf(big[nr][e], ceilf(my));
+                        const float cm = pow2_diff(m[nr][e], m1), cb = pow2_diff(big[nr][e], b1);
+                        l[nr][e] *= cm;
+                        z[nr][e] *= cm;
+                        m[nr][e] = m1;
+                        big[nr][e] = b1;
+                        fac[nr][e] = pow2_diff(m1 + kWeightUp, b1);
+#pragma unroll
+                        for (int j = 0; j < MT; j++) {
+                            o[nr][j][e] *= cb;
+                            o[nr][j][2 + e] *= cb;
+                        }
+                    }
+            }
+            uint32_t pf[NR][NS][2];
+#pragma unroll
+            for (int nr = 0; nr < NR; nr++)
+#pragma unroll
+                for (int t = 0; t < 2; t++) {
+                    float w[2];
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const float v = x[nr][2 * t + e];
+                        const float pr = v == -INFINITY ? 0.0f : ex2(v - m[nr][e]);
+                        l[nr][e] += pr;
+                        if (BV == 4 && pr != 0.0f) z[nr][e] = fmaf(pr, zv[t], z[nr][e]);
+                        w[e] = pr == 0.0f ? 0.0f : pr * fac[nr][e] * sv[t];
+                    }
+                    const uint32_t hi = f16x2(w[0], w[1]);
+                    pf[nr][0][t] = transpose8x8(hi);
+                    if constexpr (SPLIT) {
+                        const float2 back = f16x2_back(hi);
+                        pf[nr][NS - 1][t] = transpose8x8(f16x2(w[0] - back.x, w[1] - back.y));
+                    }
+                }
+            // ---- O^T += V^T P^T: tokens 2c, 2c + 1, 2c + 8, 2c + 9, dims g * D/8 .. ----
+            constexpr int VW = T::RV / 32;  // words per token (0: two bytes)
+            const uint8_t *vr = st + T::K;
+            auto v_at = [&](int i) {
+                const int row = 2 * c + (i & 1) + 8 * (i >> 1);
+                const int byte = g * (T::RV / 8);
+                return vr + row * T::RV + ((((byte >> 4) ^ v_swz<T::RV>(row)) << 4) | (byte & 15));
+            };
+            if constexpr (VW > 0) {
+                uint32_t vw[4][VW];
+#pragma unroll
+                for (int i = 0; i < 4; i++) lds_words<VW>(v_at(i), vw[i], 0);
+#pragma unroll
+                for (int w = 0; w < VW; w++) {
+                    if constexpr (BV == 8) {
+                        // interleave the bytes of tokens (0, 1) and (2, 3), then unpack pairs
+                        uint32_t a01, a23, b01, b23;
+                        asm("prmt.b32 %0, %1, %2, 0x5140;" : "=r"(a01) : "r"(vw[0][w]), "r"(vw[1][w]));
+                        asm("prmt.b32 %0, %1, %2, 0x7362;" : "=r"(a23) : "r"(vw[0][w]), "r"(vw[1][w]));
+                        asm("prmt.b32 %0, %1, %2, 0x5140;" : "=r"(b01) : "r"(vw[2][w]), "r"(vw[3][w]));
+                        asm("prmt.b32 %0, %1, %2, 0x7362;" : "=r"(b23) : "r"(vw[2][w]), "r"(vw[3][w]));
+                        uint32_t a[4], a2[4];
+                        unpack_u8(a01, a[0], a[1]);
+                        unpack_u8(b01, a[2], a[3]);
+                        unpack_u8(a23, a2[0], a2[1]);
+                        unpack_u8(b23, a2[2], a2[3]);
+#pragma unroll
+                        for (int nr = 0; nr < NR; nr++)
+#pragma unroll
+                            for (int n = 0; n < NS; n++) {
+                                mma16816(o[nr][2 * w], a, pf[nr][n]);
+                                mma16816(o[nr][2 * w + 1], a2, pf[nr][n]);
+                            }
+                    } else {
+#pragma unroll
+                        for (int half = 0; half < 2; half++) {
+                            uint32_t a01, b01;
+                            if (half == 0) {
+                                asm("prmt.b32 %0, %1, %2, 0x5410;" : "=r"(a01) : "r"(vw[0][w]), "r"(vw[1][w]));
+                                asm("prmt.b32 %0, %1, %2, 0x5410;" : "=r"(b01) : "r"(vw[2][w]), "r"(vw[3][w]));
+                            } else {
+                                asm("prmt.b32 %0, %1, %2, 0x7632;" : "=r"(a01) : "r"(vw[0][w]), "r"(vw[1][w]));
+                                asm("prmt.b32 %0, %1, %2, 0x7632;" : "=r"(b01) : "r"(vw[2][w]), "r"(vw[3][w]));
+                            }
+                            uint32_t ua[4], ub[4];
+                            unpack_u4(a01, ua);
+                            unpack_u4(b01, ub);
+                            const uint32_t a[4] = {ua[0], ua[1], ub[0], ub[1]}, a2[4] = {ua[2], ua[3], ub[2], ub[3]};
+#pragma unroll
+                            for (int nr = 0; nr < NR; nr++)
+#pragma unroll
+                                for (int n = 0; n < NS; n++) {
+                                    mma16816(o[nr][4 * w + 2 * half], a, pf[nr][n]);
+                                    mma16816(o[nr][4 * w + 2 * half + 1], a2, pf[nr][n]);
+                                }
+                        }
+                    }
+                }
+            } else {
+                // D = 32 at 4 bits: two bytes a token
+                uint32_t u[2];
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+                    u[i] = (uint32_t) * reinterpret_cast<const uint16_t *>(v_at(2 * i)) |
+                           ((uint32_t) * reinterpret_cast<const uint16_t *>(v_at(2 * i + 1)) << 16);
+                uint32_t ua[4], ub[4];
+                unpack_u4(u[0], ua);
+                unpack_u4(u[1], ub);
+                const uint32_t a[4] = {ua[0], ua[1], ub[0], ub[1]}, a2[4] = {ua[2], ua[3], ub[2], ub[3]};
+#pragma unroll
+                for (int nr = 0; nr < NR; nr++)
+#pragma unroll
+                    for (int n = 0; n < NS; n++) {
+                        mma16816(o[nr][0], a, pf[nr][n]);
+                        mma16816(o[nr][1], a2, pf[nr][n]);
+                    }
+            }
+        }
+        __syncwarp();  // every lane has read the slot that the next copy reuses
+        issue(k + kStages - 1);
+    }
+    cp_wait<0>();
+    if (fault && lane == 0) kv_report(p.fault, fault);
+
+    // ---- join the warps: records of (row, dim) in the first one's reference ----
+    __syncthreads();
+    constexpr int RS = D + 2;
+    float *rec = reinterpret_cast<float *>(smem);  // [warp][8 NR rows][D + 2]
+#pragma unroll
+    for (int nr = 0; nr < NR; nr++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            float lt = l[nr][e], zt = z[nr][e];
+#pragma unroll
+            for (int w = 4; w < 32; w <<= 1) {
+                lt += __shfl_xor_sync(0xffffffffu, lt, w);
+                zt += __shfl_xor_sync(0xffffffffu, zt, w);
+            }
+            float *r = rec + (warp * 8 * NR + 8 * nr + 2 * c + e) * RS;
+            const float back = pow2_diff(big[nr][e] - kWeightUp, m[nr][e]);
+#pragma unroll
+            for (int j = 0; j < MT; j++) {
+                r[g * (D / 8) + 2 * j] = fmaf(o[nr][j][e], back, zt);
+                r[g * (D / 8) + 2 * j + 1] = fmaf(o[nr][j][2 + e], back, zt);
+            }
+            if (g == 0) {
+                r[D] = m[nr][e];
+                r[D + 1] = lt;
+            }
+        }
+    __syncthreads();
+    const uint32_t pair = (b * p.cache.hkv + h) * p.row_tiles + rt;
+    for (uint32_t i = threadIdx.x; i < rows.n * (D / 8); i += kWarps * 32) {
+        const uint32_t r = i / (D / 8), d0 = (i % (D / 8)) * 8;
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWarps; w++) top = fmaxf(top, rec[(w * 8 * NR + r) * RS + D]);
+        float v[8] = {0, 0, 0, 0, 0, 0, 0, 0}, lsum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWarps; w++) {
+            const float *src = rec + (w * 8 * NR + r) * RS;
+            if (src[D] == -INFINITY && !(src[D + 1] != src[D + 1])) continue;
+            const float f = src[D] == top ? 1.0f : pow2_diff(src[D], top);
+            lsum = fmaf(src[D + 1], f, lsum);
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[j] = fmaf(src[d0 + j], f, v[j]);
+        }
+        if (p.nsplit > 1) {
+            float *dst = p.part + few_record(pair, R, r, p.nsplit, split) * RS;
+#pragma unroll
+            for (int j = 0; j < 8; j++) dst[d0 + j] = v[j];
+            if (d0 == 0) {
+                dst[D] = top;
+                dst[D + 1] = lsum;
+            }
+        } else {
+            const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[j] *= inv;
+            const uint32_t tok = (rows.r0 + r) / G, head = h * G + (rows.r0 + r) % G;
+            store8(p.out.data, (size_t)(seq.q0 + tok) * p.out.row_stride + head * p.out.head_stride + d0, p.out.fmt, v);
+        }
+    }
+}
+
+template <int D, int BK, int BV, int NR, bool SPLIT>
+cudaError_t launch_few_t(const KvAttnParams &p, cudaStream_t st) {
+    using T = Tile<D, BK, BV>;
+    constexpr int JOIN = kWarps * 8 * NR * (D + 2) * 4;
+    constexpr int SMEM = T::SMEM > JOIN ? T::SMEM : JOIN;
+    auto *fn = k_kv_attn_few<D, BK, BV, NR, SPLIT>;
+    if (SMEM > 48 * 1024) {
+        cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+        if (e != cudaSuccess) return e;
+    }
+    fn<<<dim3(p.nsplit * p.row_tiles, p.cache.hkv, p.batch.n_seqs), kWarps * 32, SMEM, st>>>(p);
+    return cudaGetLastError();
+}
+
+template <int D, int BK, int BV>
+cudaError_t launch_few_bits(const KvAttnParams &p, cudaStream_t st) {
+    const bool split = p.q.fmt == kFmtF32;
+    if (p.tile_rows == 8)
+        return split ? launch_few_t<D, BK, BV, 1, true>(p, st) : launch_few_t<D, BK, BV, 1, false>(p, st);
+    return split ? launch_few_t<D, BK, BV, 2, true>(p, st) : launch_few_t<D, BK, BV, 2, false>(p, st);
+}
+
+template <int D>
+cudaError_t launch_few_dim(const KvAttnParams &p, cudaStream_t st) {
+    const int bk = p.cache.bits[0], bv = p.cache.bits[1];
+    if (bk == 8) return bv == 8 ? launch_few_bits<D, 8, 8>(p, st) : launch_few_bits<D, 8, 4>(p, st);
+    return bv == 8 ? launch_few_bits<D, 4, 8>(p, st) : launch_few_bits<D, 4, 4>(p, st);
+}
+
+}  // namespace kvf
+}  // namespace nx

@@ -77,6 +77,7 @@ class CudaBackend:
         L.check(lib.nexus_cuda_backend_create(C.byref(cfg), C.byref(h)))
         self._lib = lib
         self.handle = h
+        self.device = device
 
     # -- tensor parallelism (one process per GPU) --
     def tp_init(self, rank: int, world: int, uid: bytes) -> None:
