@@ -38,6 +38,9 @@ UNITS = {
     "kernels_kv_few_d32.cu": [],
     "kernels_kv_few_d64.cu": [],
     "kernels_kv_few_d128.cu": [],
+    "kernels_kv_chunk_d32.cu": [],
+    "kernels_kv_chunk_d64.cu": [],
+    "kernels_kv_chunk_d128.cu": [],
     "kernels_kv_merge.cu": [],
     "kernels_step.cu": [],
     "kernels_peer.cu": [],

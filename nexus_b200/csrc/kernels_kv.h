@@ -45,15 +45,24 @@ struct KvAttnParams {
     // split over the context
     uint32_t nsplit, tiles_per_split;
     float *part;               // records of unfinished softmaxes (nsplit > 1)
-    uint32_t rows_limit;       // sequences of at most so many (token, head) rows per KV head
-    uint32_t tile_rows, row_tiles;  // rows of a tile (8 or 16), tiles a sequence may have
+    // sequences of at most rows_limit (token, head) rows per KV head are the
+    // few-row kernel's, the others the chunk kernel's
+    uint32_t rows_limit;
+    uint32_t tile_rows, row_tiles;  // rows of a tile (8, 16; chunk 256), tiles a sequence may have
+    int chunk;
 };
 
+// Rows of one KV head (new tokens x query heads of its group) of a sequence
+// that the few-row kernel takes.
+constexpr uint32_t kKvFewRows = 16;
+constexpr uint32_t kKvChunkRows = 256;   // rows of a chunk-kernel CTA
+constexpr uint32_t kKvChunkTile = 128;   // tokens of its key tile
 constexpr uint32_t kKvFewTile = 16;      // tokens of one warp's tile
 constexpr uint32_t kKvFewWarps = 4;
 constexpr uint32_t kKvSms = 148;
 
 cudaError_t launch_kv_attn_few(const KvAttnParams &p, cudaStream_t st);
-cudaError_t launch_kv_merge_few(const KvAttnParams &p, cudaStream_t st);
+cudaError_t launch_kv_attn_chunk(const KvAttnParams &p, cudaStream_t st);
+cudaError_t launch_kv_merge(const KvAttnParams &p, cudaStream_t st);
 
 }  // namespace nx

@@ -5,15 +5,18 @@
 // of the group (row r: token r / G, head r % G of the group), in tiles of 8 or 16.  With key j = zk_j + sk_j * kc_j (kc integer codes
 // around zero, zk = 0 for 8 bits) and likewise values:
 //   x_rj = c_r * (sk_j * (q_r . kc_j) + zk_j * sum(q_r)),  p = 2^(x - m_r)
-//   o_r  = [ 2^(R_r) sum_j (p sv_j 2^(m_r - R_r)) vc_j + sum_j p zv_j ] / sum_j p,  R_r = B_r - 14
+//   o_r  = ( sum_j (p sv_j) vc_j + sum_j p zv_j ) / sum_j p
 // so the two products run on exact small integers in f16 and everything that
 // is not an integer stays in f32.  The rounded factors are q (22 bits as f16
 // hi + lo for f32 queries, 11 bits otherwise: bf16 and f16 are exact) and the
-// weight p sv 2^(m - R) (f16; hi + lo for f32 queries).  m and B are whole
-// numbers at or above the largest x and x + log2(sv) so far: every rescaling
-// is by an exact power of two, and the weights lie below 2^14 with the largest
-// near it, whatever the scale of the values: f16 keeps its 11 bits down to
-// 2^-28 of the largest.
+// weight p sv (f16; hi + lo for f32 queries).  The reference m is a whole
+// number that puts the largest p * max(sv, |zv|) of the row at 2^9 .. 2^10 when
+// it is set and is set anew when that passes 2^15: rescaling is by exact powers
+// of two, and whatever the scale of the values the weights stay in f16's range
+// with their 11 bits down to 2^-23 of the largest.  Where the values are zero
+// only p bounds m (2^60 at most); so that p never has to make up for values of
+// an extreme magnitude, scales and zeros are first brought near one by a power
+// of two taken from the first tile whose values are not all zero.
 //
 // Bound: HBM, the visible codes and scales once (264 bytes a token and head at
 // D = 128 and 8 bits, 144 at 4).  Layout:
@@ -33,7 +36,9 @@ namespace kvf {
 
 constexpr int kWarps = kKvFewWarps;
 constexpr int kStages = 4;
-constexpr float kWeightUp = 14.0f;  // weights are kept below 2^14
+constexpr float kUp = 10.0f;       // log2 of the largest weight under a new reference
+constexpr float kLimit = 15.0f;    // log2 of the largest weight any reference stays for
+constexpr float kMaxProb = 60.0f;  // log2 of the largest p
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -107,6 +112,10 @@ __device__ __forceinline__ void lds_words(const uint8_t *p, uint32_t (&w)[N], in
     }
 }
 
+// Exponent that brings a positive magnitude near one.
+__device__ __forceinline__ int near_one(float mag) {
+    return min(120, max(-120, 127 - (int)((__float_as_uint(mag) >> 23) & 0xffu)));
+}
 // Record of row r of a (sequence, KV head) pair and split s: D floats o, then m, l.
 __host__ __device__ inline size_t few_record(uint32_t pair, uint32_t rows, uint32_t r, uint32_t nsplit, uint32_t s) {
     return ((size_t)pair * rows + r) * nsplit + s;
@@ -257,7 +266,7 @@ __global__ void __launch_bounds__(kWarps * 32, (NR == 1 && !SPLIT) ? 3 : 2) k_kv
         }
     }
 
-    float o[NR][MT][4], m[NR][2], big[NR][2], fac[NR][2], l[NR][2], z[NR][2];
+    float o[NR][MT][4], m[NR][2], l[NR][2], z[NR][2];
 #pragma unroll
     for (int nr = 0; nr < NR; nr++) {
 #pragma unroll
@@ -266,11 +275,14 @@ __global__ void __launch_bounds__(kWarps * 32, (NR == 1 && !SPLIT) ? 3 : 2) k_kv
             for (int i = 0; i < 4; i++) o[nr][j][i] = 0.0f;
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-            m[nr][e] = big[nr][e] = -INFINITY;
-            fac[nr][e] = l[nr][e] = z[nr][e] = 0.0f;
+            m[nr][e] = -INFINITY;
+            l[nr][e] = z[nr][e] = 0.0f;
         }
     }
 
+    // power of two on the values' scales and zeros (0: none of them seen so far but
+    // zero) and its reciprocal
+    float lift = 0.0f, unit = 1.0f;
     for (uint32_t k = 0; k < n_mine; k++) {
         cp_wait<kStages - 2>();
         __syncwarp();
@@ -329,7 +341,24 @@ __global__ void __launch_bounds__(kWarps * 32, (NR == 1 && !SPLIT) ? 3 : 2) k_kv
                 zk[t] = BK == 8 ? 0.0f : kscale[2 * i + 1];
                 sv[t] = BV == 8 ? vscale[i] : vscale[2 * i];
                 zv[t] = BV == 8 ? 0.0f : vscale[2 * i + 1];
-                lv[t] = lg2(sv[t]);
+            }
+            if (lift == 0.0f) {
+                float mag = 0.0f;
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+                    if (kv_needed(range, j0 + g + 8 * t, j0 + g + 8 * t + 1))
+                        mag = fmaxf(mag, fmaxf(sv[t], fabsf(zv[t])));
+                mag = warp_max(mag);
+                if (mag > 0.0f) {
+                    lift = __int_as_float((127 + near_one(mag)) << 23);
+                    unit = __int_as_float((127 - near_one(mag)) << 23);
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                sv[t] *= lift;
+                zv[t] *= lift;
+                lv[t] = lg2(BV == 8 ? sv[t] : fmaxf(sv[t], fabsf(zv[t])));
             }
             // every token of the tile seen by every row?
             const bool whole = j0 + (int)kKvFewTile - 1 <= rows.first &&
@@ -349,7 +378,7 @@ __global__ void __launch_bounds__(kWarps * 32, (NR == 1 && !SPLIT) ? 3 : 2) k_kv
                         if (!whole && !kv_visible(j0 + g + 8 * t, x_pos[nr][e], (int)p.window, (int)p.sinks))
                             v = -INFINITY;
                         x[nr][2 * t + e] = v;
-                        grow |= v > m[nr][e] || v + lv[t] > big[nr][e];
+                        grow |= v > m[nr][e] + kMaxProb || v + lv[t] > m[nr][e] + kLimit;
                     }
             if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
@@ -363,17 +392,17 @@ __global__ void __launch_bounds__(kWarps * 32, (NR == 1 && !SPLIT) ? 3 : 2) k_kv
                             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
                             my = fmaxf(my, __shfl_xor_sync(0xffffffffu, my, w));
                         }
-                        const float m1 = fmaxf(m[nr][e], ceilf(mx)), b1 = fmaxf(big[nr][e], ceilf(my));
-                        const float cm = pow2_diff(m[nr][e], m1), cb = pow2_diff(big[nr][e], b1);
+                        // (a reference is only moved up, and only where this tile needs it)
+                        float m1 = fmaxf(m[nr][e], ceilf(mx) - kMaxProb);
+                        if (my > m1 + kLimit || m1 == -INFINITY) m1 = fmaxf(m1, ceilf(my) - kUp);
+                        const float cm = m1 == m[nr][e] ? 1.0f : pow2_diff(m[nr][e], m1);
                         l[nr][e] *= cm;
                         z[nr][e] *= cm;
                         m[nr][e] = m1;
-                        big[nr][e] = b1;
-                        fac[nr][e] = pow2_diff(m1 + kWeightUp, b1);
 #pragma unroll
                         for (int j = 0; j < MT; j++) {
-                            o[nr][j][e] *= cb;
-                            o[nr][j][2 + e] *= cb;
+                            o[nr][j][e] *= cm;
+                            o[nr][j][2 + e] *= cm;
                         }
                     }
             }
@@ -389,7 +418,7 @@ __global__ void __launch_bounds__(kWarps * 32, (NR == 1 && !SPLIT) ? 3 : 2) k_kv
                         const float pr = v == -INFINITY ? 0.0f : ex2(v - m[nr][e]);
                         l[nr][e] += pr;
                         if (BV == 4 && pr != 0.0f) z[nr][e] = fmaf(pr, zv[t], z[nr][e]);
-                        w[e] = pr == 0.0f ? 0.0f : pr * fac[nr][e] * sv[t];
+                        w[e] = pr == 0.0f ? 0.0f : pr * sv[t];
                     }
                     const uint32_t hi = f16x2(w[0], w[1]);
                     pf[nr][0][t] = transpose8x8(hi);
@@ -497,11 +526,10 @@ __global__ void __launch_bounds__(kWarps * 32, (NR == 1 && !SPLIT) ? 3 : 2) k_kv
                 zt += __shfl_xor_sync(0xffffffffu, zt, w);
             }
             float *r = rec + (warp * 8 * NR + 8 * nr + 2 * c + e) * RS;
-            const float back = pow2_diff(big[nr][e] - kWeightUp, m[nr][e]);
 #pragma unroll
             for (int j = 0; j < MT; j++) {
-                r[g * (D / 8) + 2 * j] = fmaf(o[nr][j][e], back, zt);
-                r[g * (D / 8) + 2 * j + 1] = fmaf(o[nr][j][2 + e], back, zt);
+                r[g * (D / 8) + 2 * j] = (o[nr][j][e] + zt) * unit;
+                r[g * (D / 8) + 2 * j + 1] = (o[nr][j][2 + e] + zt) * unit;
             }
             if (g == 0) {
                 r[D] = m[nr][e];

@@ -119,33 +119,64 @@ int cuda_fail(nexus_cuda_backend *b, cudaError_t e) {
     return nexus_backend_fail(b, NEXUS_E_CUDA, cudaGetErrorString(e));
 }
 
-// How a call splits the context.  All of it follows from sizes and bounds, so
-// that the workspace query and a captured call agree.
-struct AttnPlan {
+// How a call divides its rows and splits the context.  All of it follows from
+// sizes and bounds, so that the workspace query and a captured call agree.
+struct Split {
     uint32_t tile_rows, row_tiles, nsplit, tiles_per_split;
     size_t bytes;
 };
+struct AttnPlan {
+    uint32_t rows_limit;  // sequences of more rows than this go to the chunk kernel
+    bool few, chunk;
+    Split f, c;
+    size_t bytes;
+};
+
+size_t part_bytes(const Split &s, uint64_t tiles, uint32_t head_dim) {
+    if (s.nsplit <= 1) return 0;
+    return ((size_t)tiles * s.tile_rows * s.nsplit * (head_dim + 2) * sizeof(float) + 15) & ~(size_t)15;
+}
 
 const char *attn_plan(const nexus_kv_cache *c, const nexus_kv_batch *t, const nexus_kv_rows *q, uint32_t window,
                       uint32_t sinks, AttnPlan *pl) {
     const uint32_t G = q->heads / c->kv_heads;
     const uint64_t rows = (uint64_t)t->max_q * G;
-    *pl = AttnPlan{8, 1, 1, 1, 0};
+    *pl = AttnPlan{};
+    pl->rows_limit = kKvFewRows;
     if (rows == 0 || t->n_seqs == 0 || q->rows == 0) return nullptr;
-    pl->tile_rows = rows <= 8 ? 8 : 16;
-    pl->row_tiles = (uint32_t)((rows + pl->tile_rows - 1) / pl->tile_rows);
-    const uint32_t toks = (pl->tile_rows + G - 1) / G + 1;
-    const uint32_t tiles = kv_tiles_bound(toks, t->max_kv, window, sinks, kKvFewTile);
-    const uint64_t pairs = (uint64_t)t->n_seqs * c->kv_heads * pl->row_tiles;
-    // parts: enough for several CTAs on every SM, none shorter than four tiles a warp
-    const uint64_t want = (kKvSms * 12 + pairs - 1) / pairs;
-    uint64_t per = (tiles + want - 1) / want;
-    if (per < 4 * kKvFewWarps) per = 4 * kKvFewWarps;
-    pl->tiles_per_split = (uint32_t)per;
-    pl->nsplit = tiles ? (uint32_t)((tiles + per - 1) / per) : 1;
-    if (pl->nsplit > 1)
-        pl->bytes = (size_t)pairs * pl->tile_rows * pl->nsplit * (c->head_dim + 2) * sizeof(float);
-    if ((uint64_t)pl->nsplit * pl->row_tiles > 0x7fffffffull) return "kv attention: too many rows";
+    pl->few = G <= kKvFewRows;
+    pl->chunk = rows > kKvFewRows;
+    const uint64_t pairs = (uint64_t)t->n_seqs * c->kv_heads;
+    if (pl->few) {
+        const uint32_t most = rows < kKvFewRows ? (uint32_t)rows : kKvFewRows;
+        pl->f.tile_rows = most <= 8 ? 8 : 16;
+        pl->f.row_tiles = (most + pl->f.tile_rows - 1) / pl->f.tile_rows;
+        const uint32_t tiles = kv_tiles_bound((most + G - 1) / G, t->max_kv, window, sinks, kKvFewTile);
+        // parts: enough for a few CTAs on every SM, none shorter than four tiles a warp
+        const uint64_t ctas = pairs * pl->f.row_tiles, want = (kKvSms * 6 + ctas - 1) / ctas;
+        uint64_t per = (tiles + want - 1) / want;
+        if (per < 4 * kKvFewWarps) per = 4 * kKvFewWarps;
+        pl->f.tiles_per_split = (uint32_t)per;
+        pl->f.nsplit = tiles ? (uint32_t)((tiles + per - 1) / per) : 1;
+        pl->f.bytes = part_bytes(pl->f, ctas, c->head_dim);
+    }
+    if (pl->chunk) {
+        pl->c.tile_rows = kKvChunkRows;
+        const uint64_t row_tiles = (rows + kKvChunkRows - 1) / kKvChunkRows;
+        const uint32_t toks = t->max_q < kKvChunkRows ? t->max_q : kKvChunkRows;
+        const uint32_t tiles = kv_tiles_bound(toks, t->max_kv, window, sinks, kKvChunkTile);
+        // one CTA an SM: parts only where the rows leave SMs without work, none
+        // shorter than four key tiles
+        const uint64_t ctas = pairs * row_tiles, want = ctas >= kKvSms ? 1 : kKvSms / ctas;
+        uint64_t per = (tiles + want - 1) / want;
+        if (per < 4) per = 4;
+        pl->c.tiles_per_split = (uint32_t)per;
+        pl->c.nsplit = tiles ? (uint32_t)((tiles + per - 1) / per) : 1;
+        if (row_tiles * pl->c.nsplit > 65535) return "kv attention: too many rows per sequence for one call";
+        pl->c.row_tiles = (uint32_t)row_tiles;
+        pl->c.bytes = part_bytes(pl->c, ctas, c->head_dim);
+    }
+    pl->bytes = pl->f.bytes + pl->c.bytes;
     return nullptr;
 }
 
@@ -251,14 +282,20 @@ extern "C" int nexus_cuda_kv_attention(nexus_cuda_backend *b, const nexus_kv_cac
     p.window = window;
     p.sinks = sinks;
     p.fault = nexus_backend_kv_fault(b);
-    p.nsplit = pl.nsplit;
-    p.tiles_per_split = pl.tiles_per_split;
-    p.tile_rows = pl.tile_rows;
-    p.row_tiles = pl.row_tiles;
-    p.rows_limit = 0xffffffffu;
-    p.part = static_cast<float *>(workspace);
-    cudaError_t r = launch_kv_attn_few(p, st);
-    if (r == cudaSuccess && p.nsplit > 1) r = launch_kv_merge_few(p, st);
+    p.rows_limit = pl.rows_limit;
+    cudaError_t r = cudaSuccess;
+    for (int chunk = 1; chunk >= 0; chunk--) {
+        if (!(chunk ? pl.chunk : pl.few)) continue;
+        const Split &s = chunk ? pl.c : pl.f;
+        p.chunk = chunk;
+        p.nsplit = s.nsplit;
+        p.tiles_per_split = s.tiles_per_split;
+        p.tile_rows = s.tile_rows;
+        p.row_tiles = s.row_tiles;
+        p.part = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + (chunk ? pl.f.bytes : 0));
+        if (r == cudaSuccess) r = chunk ? launch_kv_attn_chunk(p, st) : launch_kv_attn_few(p, st);
+        if (r == cudaSuccess && p.nsplit > 1) r = launch_kv_merge(p, st);
+    }
     return r == cudaSuccess ? NEXUS_OK : cuda_fail(b, r);
 }
 

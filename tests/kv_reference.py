@@ -53,8 +53,8 @@ def attention(q, cache, lens, table, window=0, sinks=0, scale=None):
     lens: (new tokens, cache length) per sequence, rows in order.  spread is
     sum p (|scale code| + |zero|), what a relative error of the weights can
     move the output by; reach the largest scale * sum|q||k| a row meets, what
-    an error of the scores is relative to; floor the largest p * scale of a
-    row times sum|code|, what an absolute error of the weights can move it by."""
+    an error of the scores is relative to; floor the largest p * max(scale, |zero|)
+    of a row times sum|code|, what an absolute error of the weights can move it by."""
     heads, d = q.shape[1], q.shape[2]
     hkv, page = cache.kv_heads, cache.page_tokens
     group = heads // hkv
@@ -96,7 +96,8 @@ def attention(q, cache, lens, table, window=0, sinks=0, scale=None):
                 out[rows, h * group + g] = _times(p, vv, see)
                 spread[rows, h * group + g] = _times(p, v0.abs() + vz.abs(), see)
                 sv = cache.v_scales[ids, h, tok % page][:, 0].double()
-                weight = torch.nan_to_num(torch.where(see, p * sv, torch.zeros_like(p))).amax(-1, keepdim=True)
+                mag = torch.maximum(sv, vz[:, 0].abs())
+                weight = torch.nan_to_num(torch.where(see, p * mag, torch.zeros_like(p))).amax(-1, keepdim=True)
                 code = torch.nan_to_num(v0 / sv[:, None]).abs()
                 floor[rows, h * group + g] = weight * (see.double() @ code)
                 a = (qq.abs() @ k0.abs().T + qq.abs().sum(-1, keepdim=True) * kz.abs().T) * scale
@@ -123,11 +124,11 @@ def tolerance(ref, spread, reach, floor, dtype):
       2^-23 relative to scale * sum|q||k|, that is 2^-18, in the numerator and
       in the sum: a factor 2 ln 2 < 1.5 of it in base 2;
     - exp2 and the running sums in f32: 2^-18 of everything summed;
-    - f16 has no step below 2^-24: the weights are kept below 2^14 with the
-      largest of them 2^12 or more (two roundings up to whole exponents), so
-      each of them, and the lo half for f32 queries, is off by up to
-      2^-25 / 2^12 = 2^-37 of the largest whatever its own size (a dimension
-      in which the largest weight meets code zero shows that alone)."""
+    - f16 has no step below 2^-24: the reference puts the largest
+      p * max(scale, |zero|) of a row at 2^6 or more, so each weight, and the lo
+      half for f32 queries, is off by up to 2^-25 / 2^6 = 2^-31 of the largest
+      whatever its own size (a dimension in which the largest weight meets code
+      zero shows that alone)."""
     w = 2.0 ** -21 if dtype == torch.float32 else 2.0 ** -11
     return torch.finfo(dtype).eps / 2 * ref.abs() + (w + 1.5 * 2.0 ** -18 * reach + 2.0 ** -18) * spread \
-        + 2.0 ** -36 * floor + 1e-30
+        + 2.0 ** -31 * floor + 1e-30
