@@ -38,7 +38,11 @@ using kvf::pow2_diff;
 
 constexpr int kRows = kKvChunkRows;     // rows of a CTA: two tiles of 128
 constexpr int kTok = kKvChunkTile;      // tokens of a key tile
-constexpr int kThreads = 13 * 32;
+// Four warpgroups; registers move from the copying and issuing ones to the
+// softmax (the sum stays at the launch's 512 x 128)
+constexpr int kThreads = 16 * 32;
+constexpr int kRegsSoftmax = 160, kRegsProducer = 128, kRegsIssue = 64;
+static_assert(2 * kRegsSoftmax + kRegsProducer + kRegsIssue <= 4 * 128, "more registers than the block has");
 constexpr int kBlk = 128 * 128;         // 128 rows x 64 f16, swizzled
 constexpr float kUp = 7.0f;             // a new reference puts the largest weight at 2^6 .. 2^7
 constexpr float kMaxWeight = 32768.0f;  // and it is moved when a weight passes 2^15
@@ -104,13 +108,42 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
 #pragma unroll
     for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
 }
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *v) {
+// 16 columns: started, and waited for (with every load started before).
+__device__ __forceinline__ void tmem_ld16_start(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld16_wait(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
             taddr),
         "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
         "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
         : "memory");
+}
+// Eight columns, complete on return.
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ uint32_t hmul2u(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
 }
 
 // Operand descriptor, 128-byte swizzle (bits 61-63 = 2), version 1.  K-major:
@@ -140,6 +173,15 @@ __device__ __forceinline__ bool wait_or_fault(unsigned long long *bar, unsigned 
         }
     }
     return true;
+}
+
+template <int N>
+__device__ __forceinline__ void regs_inc() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_dec() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
 template <int D, int BK, int BV, bool SPLIT>
@@ -214,6 +256,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
 
     if (warp < 8) {
         // ================= softmax: a thread owns a row =================
+        regs_inc<kRegsSoftmax>();
         const int sub = warp >> 2, wq = warp & 3;
         const uint32_t t_lane = (uint32_t)(32 * wq) << 16;
         {
@@ -278,7 +321,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
         const int first = sub ? first1 : rows.first, last = sub ? rows.last : last0;
         // rows that see nothing start with a reference of their own: they never ask for one
         float ref = pos >= 0 ? -INFINITY : 0.0f;
-        float l = 0.0f, z = 0.0f, unit = 1.0f;
+        float unit = 1.0f;
+        f2 l2 = pk(0.0f, 0.0f), z2 = l2;  // sums of p and p zv, even and odd columns apart
         const uint32_t scol = tmem + t_lane + kSCol + 128 * sub, ocol = tmem + t_lane + kOCol + D * sub;
         unsigned cnt = 0;
         bool ok = true;
@@ -300,13 +344,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
             const float zm = fmaxf(fmaxf(sl->zmax[0], sl->zmax[1]), fmaxf(sl->zmax[2], sl->zmax[3]));
             const float plim = BV == 8 ? 9.2e18f : 1.2e30f / fmaxf(zm, 1.3e11f);  // 2^63, 2^100 / |zv|
 
-            uint32_t pw[SPLIT ? 1 : 64];
-            float tl, tz;
-            // scores of columns c0 .. c0 + 3 in base 2
-            auto scores4 = [&](const float *s, int c0, f2 &x01, f2 &x23) {
+            // scores of columns c0 .. c0 + 3 in base 2, before the row's factor
+            auto scores4 = [&](const uint32_t *s, int c0, f2 &x01, f2 &x23) {
                 const float4 sk = *reinterpret_cast<const float4 *>(sl->sk + c0);
-                x01 = mul2(pk(s[0], s[1]), pk(sk.x, sk.y));
-                x23 = mul2(pk(s[2], s[3]), pk(sk.z, sk.w));
+                x01 = mul2(pk(__uint_as_float(s[0]), __uint_as_float(s[1])), pk(sk.x, sk.y));
+                x23 = mul2(pk(__uint_as_float(s[2]), __uint_as_float(s[3])), pk(sk.z, sk.w));
                 if constexpr (BK == 4) {
                     const float4 zk = *reinterpret_cast<const float4 *>(sl->zk + c0);
                     x01 = fma2(pk(zk.x, zk.y), qsum2, x01);
@@ -314,32 +356,91 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
                 }
             };
             auto seen = [&](int c) { return (c < hi && c >= lo) || (c < sink && c < hi); };
-            // weights against the current reference; true: one of them is too large for it
-            auto weigh = [&](auto masked) -> bool {
-                constexpr bool MASK = decltype(masked)::value;
-                const float rf = ref == -INFINITY ? 0.0f : ref;
-                const f2 nref = pk(-rf, -rf);
-                f2 l2 = pk(0.0f, 0.0f), z2 = pk(0.0f, 0.0f);
-                float pmax = 0.0f, wmax = 0.0f;
+            // A reference for all that has been summed and columns 16 c0 .. of this
+            // tile; what has been summed follows: l, z, the output, and the weights
+            // of this tile already written.
+            auto new_reference = [&](int c0) {
+                float mx = -INFINITY, my = -INFINITY;
+#pragma unroll 1
+                for (int c = c0; c < 8; c++) {
+                    uint32_t s[16];
+                    tmem_ld16_start(scol + 16 * c, s);
+                    tmem_ld16_wait(s);
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    float s[32];
-                    tmem_ld32(scol + 32 * c, s);
-                    uint32_t ph[16], pl[16];
-#pragma unroll
-                    for (int j = 0; j < 32; j += 4) {
-                        const int col = 32 * c + j;
+                    for (int j = 0; j < 16; j += 4) {
+                        const int col = 16 * c + j;
                         f2 x[2];
                         scores4(s + j, col, x[0], x[1]);
+                        const float4 lv = *reinterpret_cast<const float4 *>(sl->lv + col);
+#pragma unroll
+                        for (int t = 0; t < 2; t++) {
+                            float e0, e1;
+                            upk(mul2(x[t], xs2), e0, e1);
+                            if (!whole) {
+                                e0 = seen(col + 2 * t) ? e0 : -INFINITY;
+                                e1 = seen(col + 2 * t + 1) ? e1 : -INFINITY;
+                            }
+                            mx = fmaxf(mx, fmaxf(e0, e1));
+                            my = fmaxf(my, fmaxf(e0 + (t ? lv.z : lv.x), e1 + (t ? lv.w : lv.y)));
+                        }
+                    }
+                }
+                const float next = fmaxf(ref, fmaxf(ceilf(my) - kUp, ceilf(mx) - kMaxProb));
+                const float f = next == ref ? 1.0f : pow2_diff(ref, next);
+                ref = next;
+                l2 = mul2(l2, pk(f, f));
+                z2 = mul2(z2, pk(f, f));
+                if (!__any_sync(0xffffffffu, f != 1.0f)) return;
+                if (cnt > 0) {
+                    // the products so far are complete: S of this tile was issued after them
+#pragma unroll 1
+                    for (int c = 0; c < D / 16; c++) {
+                        uint32_t o[16];
+                        tmem_ld16_start(ocol + 16 * c, o);
+                        tmem_ld16_wait(o);
+#pragma unroll
+                        for (int j = 0; j < 16; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+                        tmem_st16(ocol + 16 * c, o);
+                    }
+                }
+                tmem_wait_st();
+                const uint32_t fh = f16x2(f, f);
+#pragma unroll 1
+                for (int c = 0; c < c0 * S::NQ; c++) {
+                    uint32_t w[8];
+                    tmem_ld8(scol + 8 * c, w);
+#pragma unroll
+                    for (int j = 0; j < 8; j++) w[j] = hmul2u(w[j], fh);
+                    tmem_st8(scol + 8 * c, w);
+                }
+            };
+            // The weights of 16 columns (those of `cur`, while the loads of the next
+            // into `nxt` run) against the current reference, over the scores in place.
+            auto weigh16 = [&](auto masked, int c, uint32_t(&cur)[16], uint32_t(&nxt)[16]) {
+                constexpr bool MASK = decltype(masked)::value;
+                tmem_ld16_wait(cur);
+                if (c < 7) tmem_ld16_start(scol + 16 * (c + 1), nxt);
+                uint32_t ph[8];
+                [[maybe_unused]] uint32_t pl[8];
+                f2 l_c, z_c;
+                for (bool again = false;; again = true) {
+                    const float rf = ref == -INFINITY ? 0.0f : ref;
+                    const f2 nref = pk(-rf, -rf);
+                    float pmax = 0.0f, wmax = 0.0f;
+                    l_c = z_c = pk(0.0f, 0.0f);
+#pragma unroll
+                    for (int j = 0; j < 16; j += 4) {
+                        const int col = 16 * c + j;
+                        f2 x[2];
+                        scores4(cur + j, col, x[0], x[1]);
                         const float4 sv = *reinterpret_cast<const float4 *>(sl->sv + col);
-                        float4 zv;
+                        [[maybe_unused]] float4 zv;
                         if constexpr (BV == 4) zv = *reinterpret_cast<const float4 *>(sl->zv + col);
 #pragma unroll
                         for (int t = 0; t < 2; t++) {
                             float e0, e1;
                             upk(fma2(x[t], xs2, nref), e0, e1);
                             float sv0 = t ? sv.z : sv.x, sv1 = t ? sv.w : sv.y;
-                            float p0, p1;
                             bool b0 = true, b1 = true;
                             if constexpr (MASK) {
                                 b0 = seen(col + 2 * t);
@@ -349,10 +450,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
                                 sv0 = b0 ? sv0 : 0.0f;
                                 sv1 = b1 ? sv1 : 0.0f;
                             }
-                            p0 = ex2(e0);
-                            p1 = ex2(e1);
+                            const float p0 = ex2(e0), p1 = ex2(e1);
                             const f2 pp = pk(p0, p1);
-                            l2 = add2(l2, pp);
+                            l_c = add2(l_c, pp);
                             pmax = fmaxf(pmax, fmaxf(p0, p1));
                             if constexpr (BV == 4) {
                                 float z0 = t ? zv.z : zv.x, z1 = t ? zv.w : zv.y;
@@ -360,7 +460,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
                                     z0 = b0 ? z0 : 0.0f;
                                     z1 = b1 ? z1 : 0.0f;
                                 }
-                                z2 = fma2(pp, pk(z0, z1), z2);
+                                z_c = fma2(pp, pk(z0, z1), z_c);
                             }
                             float w0, w1;
                             upk(mul2(pp, pk(sv0, sv1)), w0, w1);
@@ -373,85 +473,26 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
                             }
                         }
                     }
-                    if constexpr (SPLIT) {
-                        // in place: the columns of these tokens have been read
-                        tmem_st16(scol + 32 * c, ph);
-                        tmem_st16(scol + 32 * c + 16, pl);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 16; j++) pw[16 * c + j] = ph[j];
-                    }
+                    const bool over = ref == -INFINITY || wmax > kMaxWeight || pmax > plim;
+                    if (again || !__any_sync(0xffffffffu, over)) break;
+                    new_reference(c);
                 }
-                float a, bb;
-                upk(l2, a, bb);
-                tl = a + bb;
-                upk(z2, a, bb);
-                tz = a + bb;
-                return wmax > kMaxWeight || pmax > plim;
+                l2 = add2(l2, l_c);
+                z2 = add2(z2, z_c);
+                tmem_st8(scol + 8 * S::NQ * c, ph);
+                if constexpr (SPLIT) tmem_st8(scol + 8 * S::NQ * c + 8, pl);
             };
-            // a reference for what has been seen and this tile; everything summed so far follows
-            auto new_reference = [&](auto masked) {
-                constexpr bool MASK = decltype(masked)::value;
-                float mx = -INFINITY, my = -INFINITY;
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    float s[32];
-                    tmem_ld32(scol + 32 * c, s);
-#pragma unroll
-                    for (int j = 0; j < 32; j += 4) {
-                        const int col = 32 * c + j;
-                        f2 x[2];
-                        scores4(s + j, col, x[0], x[1]);
-                        const float4 lv = *reinterpret_cast<const float4 *>(sl->lv + col);
-#pragma unroll
-                        for (int t = 0; t < 2; t++) {
-                            float e0, e1;
-                            upk(mul2(x[t], xs2), e0, e1);
-                            if constexpr (MASK) {
-                                e0 = seen(col + 2 * t) ? e0 : -INFINITY;
-                                e1 = seen(col + 2 * t + 1) ? e1 : -INFINITY;
-                            }
-                            mx = fmaxf(mx, fmaxf(e0, e1));
-                            my = fmaxf(my, fmaxf(e0 + (t ? lv.z : lv.x), e1 + (t ? lv.w : lv.y)));
-                        }
-                    }
-                }
-                const float next = fmaxf(ref, fmaxf(ceilf(my) - kUp, ceilf(mx) - kMaxProb));
-                const float f = next == ref ? 1.0f : pow2_diff(ref, next);
-                ref = next;
-                l *= f;
-                z *= f;
-                if (cnt > 0 && __any_sync(0xffffffffu, f != 1.0f)) {
-                    // the products so far are complete: S of this tile was issued after them
-#pragma unroll 1
-                    for (int c = 0; c < D / 32; c++) {
-                        float o[32];
-                        tmem_ld32(ocol + 32 * c, o);
-                        uint32_t w[32];
-#pragma unroll
-                        for (int j = 0; j < 32; j++) w[j] = __float_as_uint(o[j] * f);
-                        tmem_st32(ocol + 32 * c, w);
-                    }
-                }
-            };
+            uint32_t sa[16], sb[16];
+            tmem_ld16_start(scol, sa);
             auto tile = [&](auto masked) {
-                // f32 queries write the weights over S as they go and so take the
-                // reference first; the others try the old one, which nearly always holds
-                bool fresh = SPLIT || __any_sync(0xffffffffu, ref == -INFINITY);
-                if (!fresh) fresh = __any_sync(0xffffffffu, weigh(masked));
-                if (fresh) {
-                    new_reference(masked);
-                    weigh(masked);
+#pragma unroll 1
+                for (int c = 0; c < 8; c += 2) {
+                    weigh16(masked, c, sa, sb);
+                    weigh16(masked, c + 1, sb, sa);
                 }
             };
             if (whole) tile(std::false_type{});
             else tile(std::true_type{});
-            l += tl;
-            z += tz;
-            if constexpr (!SPLIT) {
-#pragma unroll
-                for (int c = 0; c < 4; c++) tmem_st16(scol + 16 * c, pw + 16 * c);
-            }
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
@@ -463,6 +504,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
         ok = __all_sync(0xffffffffu, ok);
         if (ok) {
             tc_fence_after();
+            float l, z, odd;
+            upk(l2, l, odd);
+            l += odd;
+            upk(z2, z, odd);
+            z += odd;
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             const uint32_t tile_id = (b * p.cache.hkv + h) * p.row_tiles + rt;
             float *rec = p.nsplit > 1 ? p.part + kvf::few_record(tile_id, kRows, in_tile, p.nsplit, split) * (D + 2)
@@ -501,6 +547,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
         }
     } else if (warp < 12) {
         // ================= producers: codes to f16 operands =================
+        regs_dec<kRegsProducer>();
         const int pt = threadIdx.x - 256;
         constexpr int CK = RK / 16, CV = RV / 16;  // 16-byte chunks of a token = chunks of a thread
         const uint32_t *table = p.batch.table + (size_t)b * p.batch.stride;
@@ -659,7 +706,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
             cur = nxt;
         }
         if (fault) kv_report(p.fault, fault);
-    } else {
+    } else if (regs_dec<kRegsIssue>(); warp == 12) {
         // ================= MMA issue (whole warp, elected lane) =================
         constexpr uint32_t id_s = idesc_f16(kTok, false), id_o = idesc_f16(D, true);
         const uint32_t q0 = smem_u32(smem), k0 = smem_u32(smem + S::K0), v0 = smem_u32(smem + S::V0);
@@ -671,7 +718,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
             return ok;
         };
         auto mma_s = [&](int sub, uint32_t st) {
-#pragma unroll
+#pragma unroll 1
             for (int part = 0; part < S::NQ; part++)
 #pragma unroll
                 for (int ks = 0; ks < D / 16; ks++) {
@@ -682,12 +729,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
             umma_commit_w(&sfull[sub]);
         };
         auto mma_o = [&](int sub, uint32_t st) {
-#pragma unroll
-            for (int ks = 0; ks < kTok / 16; ks++) {
+#pragma unroll (SPLIT ? 2 : 8)
+            for (int ks = 0; ks < kTok / 16; ks++) {  // (two products a step for f32 queries)
                 const uint64_t bd = desc_sw128(v0 + st * S::KV + ks * 2048, kBlk);
-                const uint32_t a = tmem + kSCol + 128 * sub + (SPLIT ? 32 * (ks >> 1) + 8 * (ks & 1) : 8 * ks);
+                const uint32_t a = tmem + kSCol + 128 * sub + (SPLIT ? 16 * ks : 8 * ks);
                 umma_f16_ts_w(tmem + kOCol + D * sub, a, bd, id_o, pc[sub] != 0 || ks != 0);
-                if constexpr (SPLIT) umma_f16_ts_w(tmem + kOCol + D * sub, a + 16, bd, id_o, 1);
+                if constexpr (SPLIT) umma_f16_ts_w(tmem + kOCol + D * sub, a + 8, bd, id_o, 1);
             }
         };
         if (n > 0 && wait(&qfull, 0) && wait(&kfull[0], 0)) {
