@@ -7,14 +7,20 @@
 // kc, vc integer codes around zero (exact in f16), q as f16 (hi + lo for f32
 // queries), the weights p sv rounded to f16 (hi + lo for f32).  ref is a whole
 // number chosen so that the largest p * max(sv, |zv|) of the row lies between
-// 2^kUp-1 and 2^15; it moves only when a weight would pass 2^15, and then by
-// an exact power of two (p alone is kept below 2^60 where values are zero, and
+// 2^(kUp-1) and f16's end; it moves only when a weight would pass that, and then
+// by an exact power of two (p alone is kept below 2^60 where values are zero, and
 // the values' scales are brought near one first, as there).
 //
 // Bound: the tensor pipe (4 D flops a visible pair) and, next to it, the
 // shared-memory bandwidth that feeds it.  One CTA an SM, 256 rows (row r: token
 // r / G, head r % G) in two tiles of 128, keys in tiles of 128 tokens:
-//   warps 0-3, 4-7  softmax of row tile 0, 1 (a thread owns a row)
+//   warps 0-3, 4-7  softmax of row tile 0, 1.  Tensor memory is read in the
+//                   16x256b shape: a thread has four rows and a quarter of the
+//                   columns, so that it needs a quarter of the tokens' scales (a
+//                   thread a row, each scale read by all 32 lanes, spent 2048
+//                   cycles a tile of the shared-memory pipe on them), and the
+//                   packed weights of two neighbouring columns are the 16x128b
+//                   store's element
 //   warps 8-11      unpack the codes of a key tile into f16 operands in shared
 //                   memory (128-byte swizzle), loads one tile ahead in registers
 //   warp 12         tcgen05.mma issue: S = Q K^T (128 x 128 x D) and O += P V
@@ -41,18 +47,21 @@ constexpr int kTok = kKvChunkTile;      // tokens of a key tile
 // Four warpgroups; registers move from the copying and issuing ones to the
 // softmax (the sum stays at the launch's 512 x 128)
 constexpr int kThreads = 16 * 32;
-constexpr int kRegsSoftmax = 160, kRegsProducer = 128, kRegsIssue = 64;
+constexpr int kRegsSoftmax = 168, kRegsProducer = 120, kRegsIssue = 56;
 static_assert(2 * kRegsSoftmax + kRegsProducer + kRegsIssue <= 4 * 128, "more registers than the block has");
 constexpr int kBlk = 128 * 128;         // 128 rows x 64 f16, swizzled
-constexpr float kUp = 7.0f;             // a new reference puts the largest weight at 2^6 .. 2^7
-constexpr float kMaxWeight = 32768.0f;  // and it is moved when a weight passes 2^15
+constexpr float kUp = 4.0f;             // a new reference puts the largest weight at 2^3 .. 2^4
+constexpr float kMaxWeight = 65504.0f;  // and it is moved when a weight would leave f16
 constexpr float kMaxProb = 60.0f;       // log2 of the largest p where values are zero
 constexpr int kScaleSlots = 4;
 
-struct alignas(16) ScaleSlot {
-    float sk[kTok], zk[kTok], sv[kTok], zv[kTok], lv[kTok];  // lv = log2 max(sv, |zv|)
-    float zmax[4];                                           // largest |zv| per producer warp
-    float unit;                                              // what sv and zv were divided by
+// What the softmax needs of a key tile, by token; byte offsets in shared memory.
+struct Slot {
+    static constexpr int SK = 0, ZK = 512, SV = 1024, ZV = 1536;
+    static constexpr int LV = 2048;            // log2 max(sv, |zv|)
+    static constexpr int SMAX = 2560, ZMAX = 2576;  // largest sv, |zv| of each producer warp
+    static constexpr int UNIT = 2592;          // what sv and zv were divided by
+    static constexpr int BYTES = 2608;
 };
 
 template <int D, bool SPLIT>
@@ -63,7 +72,7 @@ struct Smem {
     static constexpr int KV = DB * kBlk;
     static constexpr int STAGES = SPLIT && D == 128 ? 1 : 2;
     static constexpr int K0 = 2 * Q_SUB, V0 = K0 + STAGES * KV, SC = V0 + STAGES * KV;
-    static constexpr int NEED = SC + kScaleSlots * (int)sizeof(ScaleSlot) + 1024;
+    static constexpr int NEED = SC + kScaleSlots * Slot::BYTES + 1024;
     // at least 120 KB: one CTA an SM, since each takes all of tensor memory
     static constexpr int TOTAL = NEED > 120 * 1024 ? NEED : 120 * 1024;
 };
@@ -92,8 +101,75 @@ __device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
     return r;
 }
 
-// 32 columns of the warp's lanes, complete on return.
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
+__device__ __forceinline__ float4 lds4(uint32_t a) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ f2 lds2(uint32_t a) {
+    f2 v;
+    asm volatile("ld.shared.b64 %0, [%1];" : "=l"(v) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ float lds1(uint32_t a) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ void sts1(uint32_t a, float v) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory"); }
+__device__ __forceinline__ void sts4(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+__device__ __forceinline__ float max4(float4 v) { return fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)); }
+// the first n of 32 bits, any n
+__device__ __forceinline__ uint32_t first_bits(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
+
+// Tensor memory, 32 lanes of a warp as rows g, g + 8 (first half) and g + 16,
+// g + 24 (second), g = lane / 4, c = lane % 4.  Loads are complete after
+// tmem_wait; `r` is tied to it so that nothing reads it before.
+//
+// 32 columns of one half: r[4 k + i] is row g + 8 (i / 2), column 8 k + 2 c + i % 2.
+__device__ __forceinline__ void tmem_ld_16x256_x4(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_16x256_x4(uint32_t taddr, const uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.16x256b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+            taddr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
+}
+// Eight columns of one half: r[2 k + i] is row g + 8 i, column 4 k + c.
+__device__ __forceinline__ void tmem_ld_16x128_x2(uint32_t taddr, uint32_t (&r)[4]) {
+    asm volatile("tcgen05.ld.sync.aligned.16x128b.x2.b32 {%0,%1,%2,%3}, [%4];\n tcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(taddr)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st_16x128_x2(uint32_t taddr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("tcgen05.st.sync.aligned.16x128b.x2.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(a), "r"(b), "r"(c), "r"(d)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st_16x128_x4(uint32_t taddr, const uint32_t (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.16x128b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(v[0]),
+                 "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
+// A lane a row: 32 columns, complete on return.
+__device__ __forceinline__ void tmem_ld_rows32(uint32_t taddr, float (&v)[32]) {
     uint32_t r[32];
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
@@ -108,37 +184,9 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
 #pragma unroll
     for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
 }
-// 16 columns: started, and waited for (with every load started before).
-__device__ __forceinline__ void tmem_ld16_start(uint32_t taddr, uint32_t (&r)[16]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr)
-        : "memory");
-}
-__device__ __forceinline__ void tmem_ld16_wait(uint32_t (&r)[16]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
-                 :
-                 : "memory");
-}
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
-            taddr),
-        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
-        : "memory");
-}
-// Eight columns, complete on return.
-__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n tcgen05.wait::ld.sync.aligned;"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-        : "r"(taddr)
-        : "memory");
+// nonzero where either half is an infinity
+__device__ __forceinline__ uint32_t inf16x2(uint32_t v) {
+    return (((v & 0x7fffu) == 0x7c00u) || ((v & 0x7fff0000u) == 0x7c000000u)) ? 1u : 0u;
 }
 __device__ __forceinline__ uint32_t hmul2u(uint32_t a, uint32_t b) {
     uint32_t r;
@@ -175,6 +223,19 @@ __device__ __forceinline__ bool wait_or_fault(unsigned long long *bar, unsigned 
     return true;
 }
 
+// The 16-byte chunks of a tile's codes over 128 producer threads: N a thread,
+// LC lanes a row, PER chunks of a lane in a row, ROWS rows between them.
+template <int D, int BITS>
+struct Chunks {
+    static constexpr int N = D * BITS / 128;
+    static constexpr int LC = N < (BITS == 8 ? 4 : 2) ? N : (BITS == 8 ? 4 : 2);
+    static constexpr int PER = N / LC, RPW = 32 / LC, ROWS = 4 * RPW;
+    __device__ static __forceinline__ uint32_t row(int it, int warp, int lane) {
+        return (it / PER) * ROWS + warp * RPW + lane / LC;
+    }
+    __device__ static __forceinline__ uint32_t col(int it, int lane) { return (it % PER) * LC + lane % LC; }
+};
+
 template <int N>
 __device__ __forceinline__ void regs_inc() {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
@@ -188,16 +249,15 @@ template <int D, int BK, int BV, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
     using S = Smem<D, SPLIT>;
     constexpr int ST = S::STAGES;
-    constexpr int RK = D * BK / 8, RV = D * BV / 8;  // code bytes of a token
     constexpr uint32_t kSCol = 0, kOCol = 256;       // per row tile: + 128, + D
     extern __shared__ uint8_t smem_raw[];
-    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    ScaleSlot *slots = reinterpret_cast<ScaleSlot *>(smem + S::SC);
+    // operand blocks start on 1024 bytes (the swizzle goes by address)
+    const uint32_t sbase = (smem_u32(smem_raw) + 1023u) & ~1023u;
     __shared__ unsigned long long kfull[2], kempty[2], vfull[2], vempty[2], scfull[kScaleSlots], sfull[2], pready[2],
         qfull, odone;
     __shared__ uint32_t tmem_base_s;
     __shared__ volatile int abort_s;
-    __shared__ float row_x[kRows], row_sum[kRows];
+    __shared__ float row_x[kRows], row_sum[kRows], row_ref[kRows];
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t split = blockIdx.y % p.nsplit, h = blockIdx.x, b = blockIdx.z;
@@ -262,7 +322,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
         {
             // this warp's 32 query rows to shared memory, D / 8 lanes a row
             constexpr int LPR = D / 8, RPP = 32 / LPR;
-            uint8_t *qs = smem + sub * S::Q_SUB;
+            const uint32_t qs = sbase + sub * S::Q_SUB;
 #pragma unroll 2
             for (int pass = 0; pass < LPR; pass++) {
                 const int rr = 32 * wq + pass * RPP + lane / LPR, cl = lane % LPR;
@@ -300,10 +360,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
                 }
 #pragma unroll
                 for (int o = LPR / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                uint8_t *dst = qs + (cl >> 3) * kBlk + rr * 128 + (((cl & 7) ^ (rr & 7)) << 4);
-                *reinterpret_cast<uint4 *>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                if constexpr (SPLIT)
-                    *reinterpret_cast<uint4 *>(dst + S::DB * kBlk) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                const uint32_t dst = qs + (cl >> 3) * kBlk + rr * 128 + (((cl & 7) ^ (rr & 7)) << 4);
+                sts4(dst, hi[0], hi[1], hi[2], hi[3]);
+                if constexpr (SPLIT) sts4(dst + S::DB * kBlk, lo[0], lo[1], lo[2], lo[3]);
                 if (cl == 0) {
                     row_x[sub * 128 + rr] = p.scale_log2 / sc;
                     row_sum[sub * 128 + rr] = sum;
@@ -313,23 +372,35 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
             __syncwarp();
             if (lane == 0) mbar_arrive(&qfull);
         }
-        const uint32_t in_tile = (uint32_t)(sub * 128 + 32 * wq + lane), r = rows.r0 + in_tile;
-        const bool valid = in_tile < rows.n;
-        const int pos = valid ? pos0 + (int)(r / G) : -1;
-        const float xs = row_x[in_tile], qsum = row_sum[in_tile];
-        const f2 xs2 = pk(xs, xs), qsum2 = pk(qsum, qsum);
-        const int first = sub ? first1 : rows.first, last = sub ? rows.last : last0;
-        // rows that see nothing start with a reference of their own: they never ask for one
-        float ref = pos >= 0 ? -INFINITY : 0.0f;
+        // this thread's rows: k = 0..3 is row 32 wq + g + 8 k of the tile
+        const int g = lane >> 2, c = lane & 3;
+        const int base_row = sub * 128 + 32 * wq;
+        int pos[4];
+        f2 xs2[4], qsum2[4], l2[4], z2[4];
+        float ref[4];
+        f2 nref2[4];  // minus the reference (0 while there is none), twice
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const uint32_t in_tile = (uint32_t)(base_row + g + 8 * k);
+            pos[k] = in_tile < rows.n ? pos0 + (int)((rows.r0 + in_tile) / G) : -1;
+            xs2[k] = pk(row_x[in_tile], row_x[in_tile]);
+            qsum2[k] = pk(row_sum[in_tile], row_sum[in_tile]);
+            // rows that see nothing start with a reference of their own: they never ask for one
+            ref[k] = pos[k] >= 0 ? -INFINITY : 0.0f;
+            nref2[k] = pk(0.0f, 0.0f);
+            l2[k] = z2[k] = pk(0.0f, 0.0f);  // sums of p and p zv of this thread's columns
+        }
+        bool unset = true;  // some reference may not be set yet
         float unit = 1.0f;
-        f2 l2 = pk(0.0f, 0.0f), z2 = l2;  // sums of p and p zv, even and odd columns apart
+        const int first = sub ? first1 : rows.first, last = sub ? rows.last : last0;
         const uint32_t scol = tmem + t_lane + kSCol + 128 * sub, ocol = tmem + t_lane + kOCol + D * sub;
+        constexpr uint32_t kHalf = 16u << 16;  // the second half of the warp's lanes
         unsigned cnt = 0;
         bool ok = true;
         for (uint32_t i = 0; i < n; i++) {
             if (!active(sub, i)) continue;
             const int j0 = (int)tile_token(i);
-            const ScaleSlot *sl = slots + (i % kScaleSlots);
+            const uint32_t sl = sbase + S::SC + (i % kScaleSlots) * Slot::BYTES;
             ok = wait_or_fault(&scfull[i % kScaleSlots], (i / kScaleSlots) & 1, &abort_s, p.fault) &&
                  wait_or_fault(&sfull[sub], cnt & 1, &abort_s, p.fault);
             ok = __all_sync(0xffffffffu, ok);
@@ -337,158 +408,225 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
             tc_fence_after();
             const bool whole = j0 + kTok - 1 <= first &&
                                (p.window == 0 || j0 > last - (int)p.window || j0 + kTok <= (int)p.sinks);
-            // visible keys of this row within the tile: [lo, hi) and [0, sink)
-            const int hi = pos - j0 + 1, lo = p.window ? max(0, pos - (int)p.window + 1) - j0 : -1;
-            const int sink = (int)min(p.sinks, 0x3fffffffu) - j0;
-            unit = sl->unit;
-            const float zm = fmaxf(fmaxf(sl->zmax[0], sl->zmax[1]), fmaxf(sl->zmax[2], sl->zmax[3]));
-            const float plim = BV == 8 ? 9.2e18f : 1.2e30f / fmaxf(zm, 1.3e11f);  // 2^63, 2^100 / |zv|
+            unit = lds1(sl + Slot::UNIT);
+            const float svmax = max4(lds4(sl + Slot::SMAX));
+            // largest sum of p over a thread's columns of a row: 2^80, and 2^100 / |zv|
+            const float plim = BV == 8 ? 1.2e24f : 1.2e30f / fmaxf(max4(lds4(sl + Slot::ZMAX)), 1e6f);
+            const float fast_lim = fminf(plim, kMaxWeight / svmax);  // sums up to this need no closer look
+            const uint32_t slc = sl + 8 * c;  // this thread's columns: 8 k + 2 c and the next
 
-            // scores of columns c0 .. c0 + 3 in base 2, before the row's factor
-            auto scores4 = [&](const uint32_t *s, int c0, f2 &x01, f2 &x23) {
-                const float4 sk = *reinterpret_cast<const float4 *>(sl->sk + c0);
-                x01 = mul2(pk(__uint_as_float(s[0]), __uint_as_float(s[1])), pk(sk.x, sk.y));
-                x23 = mul2(pk(__uint_as_float(s[2]), __uint_as_float(s[3])), pk(sk.z, sk.w));
-                if constexpr (BK == 4) {
-                    const float4 zk = *reinterpret_cast<const float4 *>(sl->zk + c0);
-                    x01 = fma2(pk(zk.x, zk.y), qsum2, x01);
-                    x23 = fma2(pk(zk.z, zk.w), qsum2, x23);
-                }
+            // bit 8 t + e: row k sees column c0 + 8 t + 2 c + e
+            auto seen = [&](int k, int c0) {
+                const int hi = pos[k] - j0 + 1, lo = p.window ? max(0, pos[k] - (int)p.window + 1) - j0 : -1;
+                const int sink = min((int)min(p.sinks, 0x3fffffffu) - j0, hi);
+                return ((first_bits(hi - c0) & ~first_bits(lo - c0)) | first_bits(sink - c0)) >> (2 * c);
             };
-            auto seen = [&](int c) { return (c < hi && c >= lo) || (c < sink && c < hi); };
-            // A reference for all that has been summed and columns 16 c0 .. of this
-            // tile; what has been summed follows: l, z, the output, and the weights
-            // of this tile already written.
-            auto new_reference = [&](int c0) {
-                float mx = -INFINITY, my = -INFINITY;
+            // the score of two columns in base 2, before the row's factor
+            auto score = [&](const uint32_t *s, f2 sk, [[maybe_unused]] f2 zk, int k) {
+                f2 x = mul2(pk(__uint_as_float(s[0]), __uint_as_float(s[1])), sk);
+                if constexpr (BK == 4) x = fma2(zk, qsum2[k], x);
+                return x;
+            };
+            // References for all that has been summed and columns 32 q0 .. of this tile;
+            // what has been summed follows: l, z, the output, and the weights of this
+            // tile already written.
+            auto new_reference = [&](int q0) {
+                float mx[4], my[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) mx[k] = my[k] = -INFINITY;
 #pragma unroll 1
-                for (int c = c0; c < 8; c++) {
-                    uint32_t s[16];
-                    tmem_ld16_start(scol + 16 * c, s);
-                    tmem_ld16_wait(s);
+                for (int q = q0; q < 4; q++) {
 #pragma unroll
-                    for (int j = 0; j < 16; j += 4) {
-                        const int col = 16 * c + j;
-                        f2 x[2];
-                        scores4(s + j, col, x[0], x[1]);
-                        const float4 lv = *reinterpret_cast<const float4 *>(sl->lv + col);
+                    for (int hh = 0; hh < 2; hh++) {
+                        uint32_t s[16];
+                        tmem_ld_16x256_x4(scol + hh * kHalf + 32 * q, s);
+                        tmem_wait(s);
 #pragma unroll
-                        for (int t = 0; t < 2; t++) {
-                            float e0, e1;
-                            upk(mul2(x[t], xs2), e0, e1);
-                            if (!whole) {
-                                e0 = seen(col + 2 * t) ? e0 : -INFINITY;
-                                e1 = seen(col + 2 * t + 1) ? e1 : -INFINITY;
+                        for (int kk = 0; kk < 2; kk++) {
+                            const int k = 2 * hh + kk;
+                            const uint32_t bits = whole ? ~0u : seen(k, 32 * q);
+#pragma unroll
+                            for (int t = 0; t < 4; t++) {
+                                const uint32_t at = slc + 4 * (32 * q + 8 * t);
+                                const f2 lv = lds2(at + Slot::LV);
+                                float e0, e1, v0, v1;
+                                upk(mul2(score(s + 4 * t + 2 * kk, lds2(at + Slot::SK), BK == 4 ? lds2(at + Slot::ZK) : 0, k),
+                                         xs2[k]),
+                                    e0, e1);
+                                upk(lv, v0, v1);
+                                e0 = bits >> (8 * t) & 1 ? e0 : -INFINITY;
+                                e1 = bits >> (8 * t + 1) & 1 ? e1 : -INFINITY;
+                                mx[k] = fmaxf(mx[k], fmaxf(e0, e1));
+                                my[k] = fmaxf(my[k], fmaxf(e0 + v0, e1 + v1));
                             }
-                            mx = fmaxf(mx, fmaxf(e0, e1));
-                            my = fmaxf(my, fmaxf(e0 + (t ? lv.z : lv.x), e1 + (t ? lv.w : lv.y)));
                         }
                     }
                 }
-                const float next = fmaxf(ref, fmaxf(ceilf(my) - kUp, ceilf(mx) - kMaxProb));
-                const float f = next == ref ? 1.0f : pow2_diff(ref, next);
-                ref = next;
-                l2 = mul2(l2, pk(f, f));
-                z2 = mul2(z2, pk(f, f));
-                if (!__any_sync(0xffffffffu, f != 1.0f)) return;
+                float f[4];
+                bool moved = false;
+                unset = false;
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+#pragma unroll
+                    for (int o = 1; o < 4; o <<= 1) {
+                        mx[k] = fmaxf(mx[k], __shfl_xor_sync(0xffffffffu, mx[k], o));
+                        my[k] = fmaxf(my[k], __shfl_xor_sync(0xffffffffu, my[k], o));
+                    }
+                    const float next = fmaxf(ref[k], fmaxf(ceilf(my[k]) - kUp, ceilf(mx[k]) - kMaxProb));
+                    f[k] = next == ref[k] ? 1.0f : pow2_diff(ref[k], next);
+                    ref[k] = next;
+                    nref2[k] = next == -INFINITY ? pk(0.0f, 0.0f) : pk(-next, -next);
+                    unset |= next == -INFINITY;
+                    moved |= f[k] != 1.0f;
+                    l2[k] = mul2(l2[k], pk(f[k], f[k]));
+                    z2[k] = mul2(z2[k], pk(f[k], f[k]));
+                }
+                if (!__any_sync(0xffffffffu, moved)) return;
                 if (cnt > 0) {
                     // the products so far are complete: S of this tile was issued after them
 #pragma unroll 1
-                    for (int c = 0; c < D / 16; c++) {
-                        uint32_t o[16];
-                        tmem_ld16_start(ocol + 16 * c, o);
-                        tmem_ld16_wait(o);
+                    for (int q = 0; q < D / 32; q++) {
 #pragma unroll
-                        for (int j = 0; j < 16; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-                        tmem_st16(ocol + 16 * c, o);
+                        for (int hh = 0; hh < 2; hh++) {
+                            uint32_t o[16];
+                            tmem_ld_16x256_x4(ocol + hh * kHalf + 32 * q, o);
+                            tmem_wait(o);
+#pragma unroll
+                            for (int j = 0; j < 16; j++)
+                                o[j] = __float_as_uint(__uint_as_float(o[j]) * f[2 * hh + (j >> 1 & 1)]);
+                            tmem_st_16x256_x4(ocol + hh * kHalf + 32 * q, o);
+                        }
                     }
                 }
                 tmem_wait_st();
-                const uint32_t fh = f16x2(f, f);
 #pragma unroll 1
-                for (int c = 0; c < c0 * S::NQ; c++) {
-                    uint32_t w[8];
-                    tmem_ld8(scol + 8 * c, w);
+                for (int q = 0; q < 2 * q0 * S::NQ; q++) {
 #pragma unroll
-                    for (int j = 0; j < 8; j++) w[j] = hmul2u(w[j], fh);
-                    tmem_st8(scol + 8 * c, w);
+                    for (int hh = 0; hh < 2; hh++) {
+                        uint32_t w[4];
+                        tmem_ld_16x128_x2(scol + hh * kHalf + 8 * q, w);
+                        const uint32_t f0 = f16x2(f[2 * hh], f[2 * hh]), f1 = f16x2(f[2 * hh + 1], f[2 * hh + 1]);
+                        tmem_st_16x128_x2(scol + hh * kHalf + 8 * q, hmul2u(w[0], f0), hmul2u(w[1], f1), hmul2u(w[2], f0),
+                                          hmul2u(w[3], f1));
+                    }
                 }
             };
-            // The weights of 16 columns (those of `cur`, while the loads of the next
-            // into `nxt` run) against the current reference, over the scores in place.
-            auto weigh16 = [&](auto masked, int c, uint32_t(&cur)[16], uint32_t(&nxt)[16]) {
-                constexpr bool MASK = decltype(masked)::value;
-                tmem_ld16_wait(cur);
-                if (c < 7) tmem_ld16_start(scol + 16 * (c + 1), nxt);
-                uint32_t ph[8];
-                [[maybe_unused]] uint32_t pl[8];
-                f2 l_c, z_c;
-                for (bool again = false;; again = true) {
-                    const float rf = ref == -INFINITY ? 0.0f : ref;
-                    const f2 nref = pk(-rf, -rf);
-                    float pmax = 0.0f, wmax = 0.0f;
-                    l_c = z_c = pk(0.0f, 0.0f);
+            // The weights of columns 32 q .. + 31 against the references, over the scores
+            // in place.  TRY: the loads of the next 32 columns run meanwhile, and where a
+            // weight would not fit nothing is written or summed and false comes back.
+            auto weigh = [&](auto masked, auto tried, int q, uint32_t(&cur)[2][16], uint32_t(&nxt)[2][16]) -> bool {
+                constexpr bool MASK = decltype(masked)::value, TRY = decltype(tried)::value;
+                tmem_wait(cur[0]);
+                tmem_wait(cur[1]);
+                if (TRY && q < 3) {
+                    tmem_ld_16x256_x4(scol + 32 * (q + 1), nxt[0]);
+                    tmem_ld_16x256_x4(scol + kHalf + 32 * (q + 1), nxt[1]);
+                }
+                uint32_t ph[2][8];
+                [[maybe_unused]] uint32_t pl[2][8];
+                f2 l_c[4];
+                [[maybe_unused]] f2 z_c[4];
+                uint32_t bits[4];
 #pragma unroll
-                    for (int j = 0; j < 16; j += 4) {
-                        const int col = 16 * c + j;
-                        f2 x[2];
-                        scores4(cur + j, col, x[0], x[1]);
-                        const float4 sv = *reinterpret_cast<const float4 *>(sl->sv + col);
-                        [[maybe_unused]] float4 zv;
-                        if constexpr (BV == 4) zv = *reinterpret_cast<const float4 *>(sl->zv + col);
+                for (int k = 0; k < 4; k++) bits[k] = MASK ? seen(k, 32 * q) : ~0u;
 #pragma unroll
-                        for (int t = 0; t < 2; t++) {
-                            float e0, e1;
-                            upk(fma2(x[t], xs2, nref), e0, e1);
-                            float sv0 = t ? sv.z : sv.x, sv1 = t ? sv.w : sv.y;
-                            bool b0 = true, b1 = true;
-                            if constexpr (MASK) {
-                                b0 = seen(col + 2 * t);
-                                b1 = seen(col + 2 * t + 1);
-                                e0 = b0 ? e0 : -INFINITY;
-                                e1 = b1 ? e1 : -INFINITY;
-                                sv0 = b0 ? sv0 : 0.0f;
-                                sv1 = b1 ? sv1 : 0.0f;
-                            }
-                            const float p0 = ex2(e0), p1 = ex2(e1);
-                            const f2 pp = pk(p0, p1);
-                            l_c = add2(l_c, pp);
-                            pmax = fmaxf(pmax, fmaxf(p0, p1));
-                            if constexpr (BV == 4) {
-                                float z0 = t ? zv.z : zv.x, z1 = t ? zv.w : zv.y;
-                                if constexpr (MASK) {
-                                    z0 = b0 ? z0 : 0.0f;
-                                    z1 = b1 ? z1 : 0.0f;
-                                }
-                                z_c = fma2(pp, pk(z0, z1), z_c);
-                            }
-                            float w0, w1;
-                            upk(mul2(pp, pk(sv0, sv1)), w0, w1);
-                            wmax = fmaxf(wmax, fmaxf(w0, w1));
-                            const uint32_t hw = f16x2(w0, w1);
-                            ph[j / 2 + t] = hw;
-                            if constexpr (SPLIT) {
-                                const float2 back = f16x2_back(hw);
-                                pl[j / 2 + t] = f16x2(w0 - back.x, w1 - back.y);
-                            }
+                for (int t = 0; t < 4; t++) {
+                    const uint32_t at = slc + 4 * (32 * q + 8 * t);
+                    const f2 sk = lds2(at + Slot::SK), sv = lds2(at + Slot::SV);
+                    [[maybe_unused]] f2 zk, zv;
+                    if constexpr (BK == 4) zk = lds2(at + Slot::ZK);
+                    else zk = sk;
+                    if constexpr (BV == 4) zv = lds2(at + Slot::ZV);
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        float e0, e1;
+                        upk(fma2(score(cur[k >> 1] + 4 * t + 2 * (k & 1), sk, zk, k), xs2[k], nref2[k]), e0, e1);
+                        if constexpr (MASK) {
+                            e0 = bits[k] >> (8 * t) & 1 ? e0 : -INFINITY;
+                            e1 = bits[k] >> (8 * t + 1) & 1 ? e1 : -INFINITY;
+                        }
+                        const f2 pp = pk(ex2(e0), ex2(e1));
+                        l_c[k] = t ? add2(l_c[k], pp) : pp;
+                        if constexpr (BV == 4) z_c[k] = t ? fma2(pp, zv, z_c[k]) : mul2(pp, zv);
+                        float w0, w1;
+                        upk(mul2(pp, sv), w0, w1);
+                        const uint32_t hw = f16x2(w0, w1);
+                        ph[k >> 1][2 * t + (k & 1)] = hw;
+                        if constexpr (SPLIT) {
+                            const float2 back = f16x2_back(hw);
+                            pl[k >> 1][2 * t + (k & 1)] = f16x2(w0 - back.x, w1 - back.y);
                         }
                     }
-                    const bool over = ref == -INFINITY || wmax > kMaxWeight || pmax > plim;
-                    if (again || !__any_sync(0xffffffffu, over)) break;
-                    new_reference(c);
                 }
-                l2 = add2(l2, l_c);
-                z2 = add2(z2, z_c);
-                tmem_st8(scol + 8 * S::NQ * c, ph);
-                if constexpr (SPLIT) tmem_st8(scol + 8 * S::NQ * c + 8, pl);
+                if constexpr (TRY) {
+                    // A weight is at most the sum of p times the largest scale.  Only where
+                    // that says nothing are the weights themselves looked at.
+                    float most = 0.0f;
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        float a, b;
+                        upk(l_c[k], a, b);
+                        most = fmaxf(most, a + b);
+                    }
+                    if (__any_sync(0xffffffffu, most > fast_lim)) {
+                        uint32_t top = 0;
+#pragma unroll
+                        for (int j = 0; j < 8; j++) top |= inf16x2(ph[0][j]) | inf16x2(ph[1][j]);
+                        if (__any_sync(0xffffffffu, most > plim || top != 0)) return false;
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    l2[k] = add2(l2[k], l_c[k]);
+                    if constexpr (BV == 4) z2[k] = add2(z2[k], z_c[k]);
+                }
+#pragma unroll
+                for (int hh = 0; hh < 2; hh++) {
+                    if constexpr (SPLIT) {
+#pragma unroll
+                        for (int u = 0; u < 2; u++) {
+                            const uint32_t at = scol + hh * kHalf + 32 * q + 16 * u;
+                            tmem_st_16x128_x2(at, ph[hh][4 * u], ph[hh][4 * u + 1], ph[hh][4 * u + 2], ph[hh][4 * u + 3]);
+                            tmem_st_16x128_x2(at + 8, pl[hh][4 * u], pl[hh][4 * u + 1], pl[hh][4 * u + 2], pl[hh][4 * u + 3]);
+                        }
+                    } else {
+                        tmem_st_16x128_x4(scol + hh * kHalf + 16 * q, ph[hh]);
+                    }
+                }
+                return true;
             };
-            uint32_t sa[16], sb[16];
-            tmem_ld16_start(scol, sa);
+            auto load = [&](int q, uint32_t(&dst)[2][16]) {
+                tmem_ld_16x256_x4(scol + 32 * q, dst[0]);
+                tmem_ld_16x256_x4(scol + kHalf + 32 * q, dst[1]);
+            };
             auto tile = [&](auto masked) {
+                const std::true_type tried{};
+                const std::false_type fits{};
+                int q = 0;  // columns from 32 q on are left to the second loop
+                if (!__any_sync(0xffffffffu, unset)) {
+                    uint32_t sa[2][16], sb[2][16];
+                    load(0, sa);
+                    q = 4;
+                    if (!weigh(masked, tried, 0, sa, sb)) q = 0;
+                    else if (!weigh(masked, tried, 1, sb, sa)) q = 1;
+                    else if (!weigh(masked, tried, 2, sa, sb)) q = 2;
+                    else if (!weigh(masked, tried, 3, sb, sa)) q = 3;
+                    if (q < 4) {
+                        // (loads must not land in registers that are put to other use)
+                        tmem_wait(sa[0]);
+                        tmem_wait(sa[1]);
+                        tmem_wait(sb[0]);
+                        tmem_wait(sb[1]);
+                    }
+                }
+                if (q < 4) {
+                    new_reference(q);
 #pragma unroll 1
-                for (int c = 0; c < 8; c += 2) {
-                    weigh16(masked, c, sa, sb);
-                    weigh16(masked, c + 1, sb, sa);
+                    for (; q < 4; q++) {
+                        uint32_t s[2][16];
+                        load(q, s);
+                        weigh(masked, fits, q, s, s);
+                    }
                 }
             };
             if (whole) tile(std::false_type{});
@@ -499,26 +637,44 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
             if (lane == 0) mbar_arrive(&pready[sub]);
             cnt++;
         }
+        // the row sums to shared memory, for the lane that writes the row
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            float lt, zt, odd;
+            upk(l2[k], lt, odd);
+            lt += odd;
+            upk(z2[k], zt, odd);
+            zt += odd;
+#pragma unroll
+            for (int o = 1; o < 4; o <<= 1) {
+                lt += __shfl_xor_sync(0xffffffffu, lt, o);
+                zt += __shfl_xor_sync(0xffffffffu, zt, o);
+            }
+            if (c == 0) {
+                row_x[base_row + g + 8 * k] = lt;
+                row_sum[base_row + g + 8 * k] = zt;
+                row_ref[base_row + g + 8 * k] = ref[k];
+            }
+        }
+        __syncwarp();
         // ---- output ----
         if (ok) ok = wait_or_fault(&odone, 0, &abort_s, p.fault);
         ok = __all_sync(0xffffffffu, ok);
         if (ok) {
             tc_fence_after();
-            float l, z, odd;
-            upk(l2, l, odd);
-            l += odd;
-            upk(z2, z, odd);
-            z += odd;
+            const uint32_t in_tile = (uint32_t)(base_row + lane), r = rows.r0 + in_tile;
+            const bool valid = in_tile < rows.n;
+            const float l = row_x[in_tile], z = row_sum[in_tile];
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             const uint32_t tile_id = (b * p.cache.hkv + h) * p.row_tiles + rt;
             float *rec = p.nsplit > 1 ? p.part + kvf::few_record(tile_id, kRows, in_tile, p.nsplit, split) * (D + 2)
                                       : nullptr;
             const size_t at = (size_t)(seq.q0 + r / G) * p.out.row_stride + (h * G + r % G) * p.out.head_stride;
 #pragma unroll 1
-            for (int c = 0; c < D / 32; c++) {
+            for (int d0 = 0; d0 < D; d0 += 32) {
                 float o[32];
                 if (cnt > 0) {
-                    tmem_ld32(ocol + 32 * c, o);
+                    tmem_ld_rows32(ocol + d0, o);
                 } else {
 #pragma unroll
                     for (int j = 0; j < 32; j++) o[j] = 0.0f;
@@ -534,22 +690,21 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
                         if (rec) {
 #pragma unroll
                             for (int e = 0; e < 8; e += 2)
-                                *reinterpret_cast<float2 *>(rec + 32 * c + 8 * u + e) = make_float2(v[e], v[e + 1]);
+                                *reinterpret_cast<float2 *>(rec + d0 + 8 * u + e) = make_float2(v[e], v[e + 1]);
                         } else {
 #pragma unroll
                             for (int e = 0; e < 8; e++) v[e] *= inv;
-                            store8(p.out.data, at + 32 * c + 8 * u, p.out.fmt, v);
+                            store8(p.out.data, at + d0 + 8 * u, p.out.fmt, v);
                         }
                     }
                 }
             }
-            if (rec && valid) *reinterpret_cast<float2 *>(rec + D) = make_float2(l == 0.0f ? -INFINITY : ref, l);
+            if (rec && valid) *reinterpret_cast<float2 *>(rec + D) = make_float2(l == 0.0f ? -INFINITY : row_ref[in_tile], l);
         }
     } else if (warp < 12) {
         // ================= producers: codes to f16 operands =================
         regs_dec<kRegsProducer>();
         const int pt = threadIdx.x - 256;
-        constexpr int CK = RK / 16, CV = RV / 16;  // 16-byte chunks of a token = chunks of a thread
         const uint32_t *table = p.batch.table + (size_t)b * p.batch.stride;
         const uint32_t mask = (1u << p.cache.shift) - 1u;
         // lane l < 8: the page of run l (16 tokens) of tile i; ~0: nothing to read there
@@ -565,17 +720,21 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
         auto slot_of = [&](uint32_t page, uint32_t j) {
             return (((size_t)page * p.cache.hkv + h) << p.cache.shift) + (j & mask);
         };
-        uint4 kr[CK], vr[CV];
+        uint4 kr[Chunks<D, BK>::N], vr[Chunks<D, BV>::N];
         float rs[4];
-        auto load_codes = [&](uint4 *dst, int chunks, const uint8_t *codes, int row_bytes, uint32_t pages, uint32_t i) {
+        // A thread's chunks of 16 bytes: LC lanes a row, so that the eight lanes of
+        // a store phase write eight different 16-byte columns of the swizzled rows
+        auto load_codes = [&](auto bits_c, uint4 *dst, const uint8_t *codes, uint32_t pages, uint32_t i) {
+            using C = Chunks<D, decltype(bits_c)::value>;
             const uint32_t j0 = tile_token(i);
 #pragma unroll
-            for (int it = 0; it < chunks; it++) {
-                const uint32_t id = it * 128 + pt, row = id / chunks, col = id % chunks;
+            for (int it = 0; it < C::N; it++) {
+                const uint32_t row = C::row(it, warp - 8, lane), col = C::col(it, lane);
                 const uint32_t page = __shfl_sync(0xffffffffu, pages, row >> 4);
                 dst[it] = make_uint4(0u, 0u, 0u, 0u);
                 if (page != ~0u)
-                    dst[it] = ld_stream(reinterpret_cast<const uint4 *>(codes + slot_of(page, j0 + row) * row_bytes + col * 16));
+                    dst[it] = ld_stream(
+                        reinterpret_cast<const uint4 *>(codes + slot_of(page, j0 + row) * (C::N * 16) + col * 16));
             }
         };
         auto load_scales = [&](uint32_t pages, uint32_t i) {
@@ -600,56 +759,50 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
                 }
             }
         };
-        auto unpack8 = [](const uint4 &v, uint8_t *base, int row, int col) {
-            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-            uint4 o[2];
-            uint32_t *ow = reinterpret_cast<uint32_t *>(o);
+        auto store_codes = [&](auto bits_c, const uint4 *src, uint32_t base) {
+            constexpr int BITS = decltype(bits_c)::value;
+            using C = Chunks<D, BITS>;
+            const uint32_t row0 = C::row(0, warp - 8, lane), at = base + row0 * 128;
+            const uint32_t c16 = ((uint32_t)(lane % C::LC) * (BITS == 8 ? 2 : 4) ^ (row0 & 7)) << 4;
 #pragma unroll
-            for (int k = 0; k < 4; k++) unpack_u8(w[k], ow[2 * k], ow[2 * k + 1]);
-            // lanes of the second 64 dims write their odd chunk first: no two of a
-            // quarter warp in one bank
-            const int odd = (col >> 2) & 1;
+            for (int it = 0; it < C::N; it++) {
+                const uint32_t w[4] = {src[it].x, src[it].y, src[it].z, src[it].w};
+                const uint32_t dst = at + (it % C::PER) * kBlk + (it / C::PER) * C::ROWS * 128;
+                if constexpr (BITS == 8) {
+                    uint32_t u[8];
 #pragma unroll
-            for (int k = 0; k < 2; k++) {
-                const int ch = 2 * col + (k ^ odd);
-                const uint4 val = (k ^ odd) ? o[1] : o[0];
-                *reinterpret_cast<uint4 *>(base + (ch >> 3) * kBlk + row * 128 + (((ch & 7) ^ (row & 7)) << 4)) = val;
+                    for (int k = 0; k < 4; k++) unpack_u8(w[k], u[2 * k], u[2 * k + 1]);
+                    sts4(dst + c16, u[0], u[1], u[2], u[3]);
+                    sts4(dst + (c16 ^ 16u), u[4], u[5], u[6], u[7]);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        uint32_t u[4];
+                        unpack_u4(w[k], u);
+                        sts4(dst + (c16 ^ (16u * k)), u[0], u[1], u[2], u[3]);
+                    }
+                }
             }
         };
-        auto unpack4 = [](const uint4 &v, uint8_t *base, int row, int col) {
-            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                uint32_t u[4];
-                unpack_u4(w[k], u);
-                const int ch = 4 * col + k;
-                *reinterpret_cast<uint4 *>(base + (ch >> 3) * kBlk + row * 128 + (((ch & 7) ^ (row & 7)) << 4)) =
-                    make_uint4(u[0], u[1], u[2], u[3]);
-            }
-        };
+        const std::integral_constant<int, BK> kbits{};
+        const std::integral_constant<int, BV> vbits{};
         // power of two on the values' scales and zeros (0: none of them seen so far
         // but zero), the same in all four warps, and its reciprocal
         float lift = 0.0f, unit = 1.0f;
         uint32_t cur = run_pages(0);
         if (n > 0) {
-            load_codes(kr, CK, p.cache.codes[0], RK, cur, 0);
+            load_codes(kbits, kr, p.cache.codes[0], cur, 0);
             load_scales(cur, 0);
         }
         bool ok = true;
         for (uint32_t i = 0; i < n; i++) {
             const uint32_t st = i % ST, ph = (i / ST) & 1;
-            load_codes(vr, CV, p.cache.codes[1], RV, cur, i);
+            load_codes(vbits, vr, p.cache.codes[1], cur, i);
             const uint32_t nxt = run_pages(i + 1);
             ok = __all_sync(0xffffffffu, wait_or_fault(&kempty[st], ph ^ 1, &abort_s, p.fault));
             if (!ok) break;
-            uint8_t *kb = smem + S::K0 + st * S::KV;
-#pragma unroll
-            for (int it = 0; it < CK; it++) {
-                const int id = it * 128 + pt;
-                if constexpr (BK == 8) unpack8(kr[it], kb, id / CK, id % CK);
-                else unpack4(kr[it], kb, id / CK, id % CK);
-            }
-            ScaleSlot *sl = slots + (i % kScaleSlots);
+            store_codes(kbits, kr, sbase + S::K0 + st * S::KV);
+            const uint32_t sl = sbase + S::SC + (i % kScaleSlots) * Slot::BYTES;
             if (lift == 0.0f) {
                 // every warp looks at the whole tile: no wait between warps
                 float mag = 0.0f;
@@ -673,14 +826,23 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
             }
             rs[2] *= lift;
             rs[3] *= lift;
-            sl->sk[pt] = rs[0];
-            sl->sv[pt] = rs[2];
-            sl->lv[pt] = lg2(fmaxf(rs[2], fabsf(rs[3])));
-            if constexpr (BK == 4) sl->zk[pt] = rs[1];
-            if constexpr (BV == 4) sl->zv[pt] = rs[3];
-            const float zm = BV == 4 ? warp_max(fabsf(rs[3])) : 0.0f;
-            if (lane == 0) sl->zmax[warp - 8] = zm;
-            if (pt == 0) sl->unit = unit;
+            if (!(fabsf(rs[2]) <= 3.4e38f && fabsf(rs[3]) <= 3.4e38f)) {
+                // not a number: the score says so to the rows that see the token, the
+                // others multiply its value by zero
+                rs[0] = kv_nan();
+                rs[2] = rs[3] = 0.0f;
+            }
+            sts1(sl + Slot::SK + 4 * pt, rs[0]);
+            sts1(sl + Slot::SV + 4 * pt, rs[2]);
+            sts1(sl + Slot::LV + 4 * pt, lg2(fmaxf(rs[2], fabsf(rs[3]))));
+            if constexpr (BK == 4) sts1(sl + Slot::ZK + 4 * pt, rs[1]);
+            if constexpr (BV == 4) sts1(sl + Slot::ZV + 4 * pt, rs[3]);
+            const float sm = warp_max(rs[2]), zm = BV == 4 ? warp_max(fabsf(rs[3])) : 0.0f;
+            if (lane == 0) {
+                sts1(sl + Slot::SMAX + 4 * (warp - 8), sm);
+                sts1(sl + Slot::ZMAX + 4 * (warp - 8), zm);
+            }
+            if (pt == 0) sts1(sl + Slot::UNIT, unit);
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
@@ -688,18 +850,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
                 mbar_arrive(&kfull[st]);
             }
             if (i + 1 < n) {
-                load_codes(kr, CK, p.cache.codes[0], RK, nxt, i + 1);
+                load_codes(kbits, kr, p.cache.codes[0], nxt, i + 1);
                 load_scales(nxt, i + 1);
             }
             ok = __all_sync(0xffffffffu, wait_or_fault(&vempty[st], ph ^ 1, &abort_s, p.fault));
             if (!ok) break;
-            uint8_t *vb = smem + S::V0 + st * S::KV;
-#pragma unroll
-            for (int it = 0; it < CV; it++) {
-                const int id = it * 128 + pt;
-                if constexpr (BV == 8) unpack8(vr[it], vb, id / CV, id % CV);
-                else unpack4(vr[it], vb, id / CV, id % CV);
-            }
+            store_codes(vbits, vr, sbase + S::V0 + st * S::KV);
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&vfull[st]);
@@ -709,7 +865,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
     } else if (regs_dec<kRegsIssue>(); warp == 12) {
         // ================= MMA issue (whole warp, elected lane) =================
         constexpr uint32_t id_s = idesc_f16(kTok, false), id_o = idesc_f16(D, true);
-        const uint32_t q0 = smem_u32(smem), k0 = smem_u32(smem + S::K0), v0 = smem_u32(smem + S::V0);
+        const uint32_t q0 = sbase, k0 = sbase + S::K0, v0 = sbase + S::V0;
         unsigned pc[2] = {0, 0};  // products of P done so far, per row tile
         bool ok = true;
         auto wait = [&](unsigned long long *bar, unsigned parity) {

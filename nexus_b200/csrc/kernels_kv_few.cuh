@@ -112,9 +112,9 @@ __device__ __forceinline__ void lds_words(const uint8_t *p, uint32_t (&w)[N], in
     }
 }
 
-// Exponent that brings a positive magnitude near one.
+// Exponent that brings a positive magnitude near one, or within p's 2^60 of it.
 __device__ __forceinline__ int near_one(float mag) {
-    return min(120, max(-120, 127 - (int)((__float_as_uint(mag) >> 23) & 0xffu)));
+    return min(60, max(-60, 127 - (int)((__float_as_uint(mag) >> 23) & 0xffu)));
 }
 // Record of row r of a (sequence, KV head) pair and split s: D floats o, then m, l.
 __host__ __device__ inline size_t few_record(uint32_t pair, uint32_t rows, uint32_t r, uint32_t nsplit, uint32_t s) {

@@ -125,10 +125,10 @@ def tolerance(ref, spread, reach, floor, dtype):
       in the sum: a factor 2 ln 2 < 1.5 of it in base 2;
     - exp2 and the running sums in f32: 2^-18 of everything summed;
     - f16 has no step below 2^-24: the reference puts the largest
-      p * max(scale, |zero|) of a row at 2^6 or more, so each weight, and the lo
-      half for f32 queries, is off by up to 2^-25 / 2^6 = 2^-31 of the largest
+      p * max(scale, |zero|) of a row at 2^3 or more, so each weight, and the lo
+      half for f32 queries, is off by up to 2^-25 / 2^3 = 2^-28 of the largest
       whatever its own size (a dimension in which the largest weight meets code
       zero shows that alone)."""
     w = 2.0 ** -21 if dtype == torch.float32 else 2.0 ** -11
     return torch.finfo(dtype).eps / 2 * ref.abs() + (w + 1.5 * 2.0 ** -18 * reach + 2.0 ** -18) * spread \
-        + 2.0 ** -31 * floor + 1e-30
+        + 2.0 ** -28 * floor + 1e-30
