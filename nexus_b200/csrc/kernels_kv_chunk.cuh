@@ -168,6 +168,19 @@ __device__ __forceinline__ void tmem_st_16x128_x4(uint32_t taddr, const uint32_t
                  "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
                  : "memory");
 }
+// The stores and sums of the common path, left out where `on` (the same in all
+// lanes) is zero: no branch, so that a tile is one stretch of code and the tail
+// of a quarter of it runs under the head of the next.
+__device__ __forceinline__ void tmem_st_16x128_x4_if(unsigned on, uint32_t taddr, const uint32_t (&v)[8]) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.u32 p, %9, 0;\n"
+        " @p tcgen05.st.sync.aligned.16x128b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n}\n" ::"r"(taddr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(on)
+        : "memory");
+}
+__device__ __forceinline__ void add2_if(unsigned on, f2 &a, f2 b) {
+    asm("{\n .reg .pred p;\n setp.ne.u32 p, %2, 0;\n @p add.rn.f32x2 %0, %0, %1;\n}\n" : "+l"(a) : "l"(b), "r"(on));
+}
 // A lane a row: 32 columns, complete on return.
 __device__ __forceinline__ void tmem_ld_rows32(uint32_t taddr, float (&v)[32]) {
     uint32_t r[32];
@@ -183,10 +196,6 @@ __device__ __forceinline__ void tmem_ld_rows32(uint32_t taddr, float (&v)[32]) {
         : "memory");
 #pragma unroll
     for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
-}
-// nonzero where either half is an infinity
-__device__ __forceinline__ uint32_t inf16x2(uint32_t v) {
-    return (((v & 0x7fffu) == 0x7c00u) || ((v & 0x7fff0000u) == 0x7c000000u)) ? 1u : 0u;
 }
 __device__ __forceinline__ uint32_t hmul2u(uint32_t a, uint32_t b) {
     uint32_t r;
@@ -412,7 +421,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
             const float svmax = max4(lds4(sl + Slot::SMAX));
             // largest sum of p over a thread's columns of a row: 2^80, and 2^100 / |zv|
             const float plim = BV == 8 ? 1.2e24f : 1.2e30f / fmaxf(max4(lds4(sl + Slot::ZMAX)), 1e6f);
-            const float fast_lim = fminf(plim, kMaxWeight / svmax);  // sums up to this need no closer look
+            const float fast_lim = fminf(plim, kMaxWeight / svmax);  // sums of p up to this keep every weight in f16
             const uint32_t slc = sl + 8 * c;  // this thread's columns: 8 k + 2 c and the next
 
             // bit 8 t + e: row k sees column c0 + 8 t + 2 c + e
@@ -511,21 +520,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
                     }
                 }
             };
-            // The weights of columns 32 q .. + 31 against the references, over the scores
-            // in place.  TRY: the loads of the next 32 columns run meanwhile, and where a
-            // weight would not fit nothing is written or summed and false comes back.
-            auto weigh = [&](auto masked, auto tried, int q, uint32_t(&cur)[2][16], uint32_t(&nxt)[2][16]) -> bool {
-                constexpr bool MASK = decltype(masked)::value, TRY = decltype(tried)::value;
-                tmem_wait(cur[0]);
-                tmem_wait(cur[1]);
-                if (TRY && q < 3) {
-                    tmem_ld_16x256_x4(scol + 32 * (q + 1), nxt[0]);
-                    tmem_ld_16x256_x4(scol + kHalf + 32 * (q + 1), nxt[1]);
-                }
-                uint32_t ph[2][8];
-                [[maybe_unused]] uint32_t pl[2][8];
-                f2 l_c[4];
-                [[maybe_unused]] f2 z_c[4];
+            // The weights of columns 32 q .. + 31 against the references, and their sums.
+            // Returns the largest of the sums of p.
+            auto weigh = [&](auto masked, int q, const uint32_t(&cur)[2][16], uint32_t(&ph)[2][8], uint32_t(&pl)[2][8],
+                             f2(&l_c)[4], f2(&z_c)[4]) -> float {
+                constexpr bool MASK = decltype(masked)::value;
                 uint32_t bits[4];
 #pragma unroll
                 for (int k = 0; k < 4; k++) bits[k] = MASK ? seen(k, 32 * q) : ~0u;
@@ -558,74 +557,83 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
                         }
                     }
                 }
-                if constexpr (TRY) {
-                    // A weight is at most the sum of p times the largest scale.  Only where
-                    // that says nothing are the weights themselves looked at.
-                    float most = 0.0f;
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        float a, b;
-                        upk(l_c[k], a, b);
-                        most = fmaxf(most, a + b);
-                    }
-                    if (__any_sync(0xffffffffu, most > fast_lim)) {
-                        uint32_t top = 0;
-#pragma unroll
-                        for (int j = 0; j < 8; j++) top |= inf16x2(ph[0][j]) | inf16x2(ph[1][j]);
-                        if (__any_sync(0xffffffffu, most > plim || top != 0)) return false;
-                    }
-                }
+                float sum[4];
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
-                    l2[k] = add2(l2[k], l_c[k]);
-                    if constexpr (BV == 4) z2[k] = add2(z2[k], z_c[k]);
+                    float a, b;
+                    upk(l_c[k], a, b);
+                    sum[k] = a + b;
+                }
+                return fmaxf(fmaxf(sum[0], sum[1]), fmaxf(sum[2], sum[3]));
+            };
+            // Writes the weights over the scores and adds the sums, where `on`.
+            auto keep = [&](unsigned on, int q, const uint32_t(&ph)[2][8], const uint32_t(&pl)[2][8], const f2(&l_c)[4],
+                            const f2(&z_c)[4]) {
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    add2_if(on, l2[k], l_c[k]);
+                    if constexpr (BV == 4) add2_if(on, z2[k], z_c[k]);
                 }
 #pragma unroll
                 for (int hh = 0; hh < 2; hh++) {
                     if constexpr (SPLIT) {
+                        // 16 tokens: eight columns of hi, eight of lo
+                        uint32_t w[2][8];
 #pragma unroll
-                        for (int u = 0; u < 2; u++) {
-                            const uint32_t at = scol + hh * kHalf + 32 * q + 16 * u;
-                            tmem_st_16x128_x2(at, ph[hh][4 * u], ph[hh][4 * u + 1], ph[hh][4 * u + 2], ph[hh][4 * u + 3]);
-                            tmem_st_16x128_x2(at + 8, pl[hh][4 * u], pl[hh][4 * u + 1], pl[hh][4 * u + 2], pl[hh][4 * u + 3]);
+                        for (int e = 0; e < 4; e++) {
+                            w[0][e] = ph[hh][e];
+                            w[0][4 + e] = pl[hh][e];
+                            w[1][e] = ph[hh][4 + e];
+                            w[1][4 + e] = pl[hh][4 + e];
                         }
+                        tmem_st_16x128_x4_if(on, scol + hh * kHalf + 32 * q, w[0]);
+                        tmem_st_16x128_x4_if(on, scol + hh * kHalf + 32 * q + 16, w[1]);
                     } else {
-                        tmem_st_16x128_x4(scol + hh * kHalf + 16 * q, ph[hh]);
+                        tmem_st_16x128_x4_if(on, scol + hh * kHalf + 16 * q, ph[hh]);
                     }
                 }
-                return true;
             };
             auto load = [&](int q, uint32_t(&dst)[2][16]) {
                 tmem_ld_16x256_x4(scol + 32 * q, dst[0]);
                 tmem_ld_16x256_x4(scol + kHalf + 32 * q, dst[1]);
             };
             auto tile = [&](auto masked) {
-                const std::true_type tried{};
-                const std::false_type fits{};
-                int q = 0;  // columns from 32 q on are left to the second loop
+                // Common path: the old references hold for the whole tile.  A weight is at
+                // most the sum of p times the largest scale; from the first quarter where
+                // that says nothing on, the second loop takes over.
+                int q = 0;
                 if (!__any_sync(0xffffffffu, unset)) {
-                    uint32_t sa[2][16], sb[2][16];
-                    load(0, sa);
-                    q = 4;
-                    if (!weigh(masked, tried, 0, sa, sb)) q = 0;
-                    else if (!weigh(masked, tried, 1, sb, sa)) q = 1;
-                    else if (!weigh(masked, tried, 2, sa, sb)) q = 2;
-                    else if (!weigh(masked, tried, 3, sb, sa)) q = 3;
-                    if (q < 4) {
-                        // (loads must not land in registers that are put to other use)
-                        tmem_wait(sa[0]);
-                        tmem_wait(sa[1]);
-                        tmem_wait(sb[0]);
-                        tmem_wait(sb[1]);
+                    uint32_t s[2][2][16];
+                    unsigned on = 1;
+                    load(0, s[0]);
+#pragma unroll
+                    for (int u = 0; u < 4; u++) {
+                        uint32_t ph[2][8];
+                        [[maybe_unused]] uint32_t pl[2][8];
+                        f2 l_c[4];
+                        [[maybe_unused]] f2 z_c[4];
+                        tmem_wait(s[u & 1][0]);
+                        tmem_wait(s[u & 1][1]);
+                        if (u < 3) load(u + 1, s[(u + 1) & 1]);
+                        const float most = weigh(masked, u, s[u & 1], ph, pl, l_c, z_c);
+                        on &= __any_sync(0xffffffffu, most > fast_lim) ? 0u : 1u;
+                        keep(on, u, ph, pl, l_c, z_c);
+                        q += (int)on;
                     }
                 }
                 if (q < 4) {
                     new_reference(q);
 #pragma unroll 1
                     for (; q < 4; q++) {
-                        uint32_t s[2][16];
+                        uint32_t s[2][16], ph[2][8];
+                        [[maybe_unused]] uint32_t pl[2][8];
+                        f2 l_c[4];
+                        [[maybe_unused]] f2 z_c[4];
                         load(q, s);
-                        weigh(masked, fits, q, s, s);
+                        tmem_wait(s[0]);
+                        tmem_wait(s[1]);
+                        weigh(masked, q, s, ph, pl, l_c, z_c);
+                        keep(1u, q, ph, pl, l_c, z_c);
                     }
                 }
             };
