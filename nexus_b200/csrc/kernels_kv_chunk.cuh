@@ -21,8 +21,9 @@
 //                   cycles a tile of the shared-memory pipe on them), and the
 //                   packed weights of two neighbouring columns are the 16x128b
 //                   store's element
-//   warps 8-11      unpack the codes of a key tile into f16 operands in shared
-//                   memory (128-byte swizzle), loads one tile ahead in registers
+//   warps 8-9, 10-11  unpack the key and the value codes of a tile into f16
+//                   operands in shared memory (128-byte swizzle); the next tile's
+//                   codes are on their way in registers meanwhile
 //   warp 12         tcgen05.mma issue: S = Q K^T (128 x 128 x D) and O += P V
 // S and O of both tiles fill tensor memory; P overwrites S in place.  While the
 // softmax of one tile runs, the tensor pipe works for the other.  Keys come in
@@ -47,8 +48,8 @@ constexpr int kTok = kKvChunkTile;      // tokens of a key tile
 // Four warpgroups; registers move from the copying and issuing ones to the
 // softmax (the sum stays at the launch's 512 x 128)
 constexpr int kThreads = 16 * 32;
-constexpr int kRegsSoftmax = 168, kRegsProducer = 120, kRegsIssue = 56;
-static_assert(2 * kRegsSoftmax + kRegsProducer + kRegsIssue <= 4 * 128, "more registers than the block has");
+constexpr int kRegsLaunch = 128, kRegsSoftmax = 160, kRegsProducer = 120, kRegsIssue = 72;
+static_assert(2 * kRegsSoftmax + kRegsProducer + kRegsIssue <= 4 * kRegsLaunch && kThreads * kRegsLaunch <= 65536, "more registers than the block has");
 constexpr int kBlk = 128 * 128;         // 128 rows x 64 f16, swizzled
 constexpr float kUp = 4.0f;             // a new reference puts the largest weight at 2^3 .. 2^4
 constexpr float kMaxWeight = 65504.0f;  // and it is moved when a weight would leave f16
@@ -59,7 +60,7 @@ constexpr int kScaleSlots = 4;
 struct Slot {
     static constexpr int SK = 0, ZK = 512, SV = 1024, ZV = 1536;
     static constexpr int LV = 2048;            // log2 max(sv, |zv|)
-    static constexpr int SMAX = 2560, ZMAX = 2576;  // largest sv, |zv| of each producer warp
+    static constexpr int SMAX = 2560, ZMAX = 2576;  // largest sv, |zv| of each quarter of the tokens
     static constexpr int UNIT = 2592;          // what sv and zv were divided by
     static constexpr int BYTES = 2608;
 };
@@ -163,14 +164,8 @@ __device__ __forceinline__ void tmem_st_16x128_x2(uint32_t taddr, uint32_t a, ui
     asm volatile("tcgen05.st.sync.aligned.16x128b.x2.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(a), "r"(b), "r"(c), "r"(d)
                  : "memory");
 }
-__device__ __forceinline__ void tmem_st_16x128_x4(uint32_t taddr, const uint32_t (&v)[8]) {
-    asm volatile("tcgen05.st.sync.aligned.16x128b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(v[0]),
-                 "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-                 : "memory");
-}
 // The stores and sums of the common path, left out where `on` (the same in all
-// lanes) is zero: no branch, so that a tile is one stretch of code and the tail
-// of a quarter of it runs under the head of the next.
+// lanes) is zero, without a branch.
 __device__ __forceinline__ void tmem_st_16x128_x4_if(unsigned on, uint32_t taddr, const uint32_t (&v)[8]) {
     asm volatile(
         "{\n .reg .pred p;\n setp.ne.u32 p, %9, 0;\n"
@@ -232,26 +227,25 @@ __device__ __forceinline__ bool wait_or_fault(unsigned long long *bar, unsigned 
     return true;
 }
 
-// The 16-byte chunks of a tile's codes over 128 producer threads: N a thread,
-// LC lanes a row, PER chunks of a lane in a row, ROWS rows between them.
+// The 16-byte chunks of a tile's codes over two producer warps: CPR a row, N a
+// thread, LC lanes a row, PER chunks of a lane in a row, ROWS rows between them.
 template <int D, int BITS>
 struct Chunks {
-    static constexpr int N = D * BITS / 128;
-    static constexpr int LC = N < (BITS == 8 ? 4 : 2) ? N : (BITS == 8 ? 4 : 2);
-    static constexpr int PER = N / LC, RPW = 32 / LC, ROWS = 4 * RPW;
+    static constexpr int CPR = D * BITS / 128, N = 2 * CPR;
+    static constexpr int LC = CPR < (BITS == 8 ? 4 : 2) ? CPR : (BITS == 8 ? 4 : 2);
+    static constexpr int PER = CPR / LC, RPW = 32 / LC, ROWS = 2 * RPW;
     __device__ static __forceinline__ uint32_t row(int it, int warp, int lane) {
         return (it / PER) * ROWS + warp * RPW + lane / LC;
     }
     __device__ static __forceinline__ uint32_t col(int it, int lane) { return (it % PER) * LC + lane % LC; }
 };
 
+// The warpgroup's registers a thread from the launch's 128 to N (each form of the
+// instruction goes one way only).
 template <int N>
-__device__ __forceinline__ void regs_inc() {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-}
-template <int N>
-__device__ __forceinline__ void regs_dec() {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+__device__ __forceinline__ void set_regs() {
+    if constexpr (N > kRegsLaunch) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+    if constexpr (N < kRegsLaunch) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
 template <int D, int BK, int BV, bool SPLIT>
@@ -300,14 +294,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; i++) {
-            mbar_init(&kfull[i], 4);
+            mbar_init(&kfull[i], 2);
             mbar_init(&kempty[i], 1);
-            mbar_init(&vfull[i], 4);
+            mbar_init(&vfull[i], 2);
             mbar_init(&vempty[i], 1);
             mbar_init(&sfull[i], 1);
             mbar_init(&pready[i], 4);
         }
-        for (int i = 0; i < kScaleSlots; i++) mbar_init(&scfull[i], 4);
+        for (int i = 0; i < kScaleSlots; i++) mbar_init(&scfull[i], 2);
         mbar_init(&qfull, 8);
         mbar_init(&odone, 1);
         abort_s = 0;
@@ -325,22 +319,49 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
 
     if (warp < 8) {
         // ================= softmax: a thread owns a row =================
-        regs_inc<kRegsSoftmax>();
+        set_regs<kRegsSoftmax>();
         const int sub = warp >> 2, wq = warp & 3;
         const uint32_t t_lane = (uint32_t)(32 * wq) << 16;
         {
-            // this warp's 32 query rows to shared memory, D / 8 lanes a row
+            // This warp's 32 query rows to shared memory, D / 8 lanes a row: first as they
+            // are, every copy in flight at once, each lane's 16 bytes where its f16 will
+            // stand (f32: the two halves where hi and lo will), then converted in place.
+            // Rolled loops: the code is cold in every CTA, and fetching eight passes
+            // unrolled took 8 us.
             constexpr int LPR = D / 8, RPP = 32 / LPR;
-            const uint32_t qs = sbase + sub * S::Q_SUB;
-#pragma unroll 2
+            const int cl = lane % LPR;
+            const uint32_t qs = sbase + sub * S::Q_SUB + (cl >> 3) * kBlk;
+            auto place = [&](int rr) { return qs + rr * 128 + (((cl & 7) ^ (rr & 7)) << 4); };
+#pragma unroll 1
             for (int pass = 0; pass < LPR; pass++) {
-                const int rr = 32 * wq + pass * RPP + lane / LPR, cl = lane % LPR;
-                const uint32_t in_tile = (uint32_t)(sub * 128 + rr), r = rows.r0 + in_tile;
-                float q[8];
-                if (in_tile < rows.n) {
-                    load8(p.q.data, (size_t)(seq.q0 + r / G) * p.q.row_stride + (h * G + r % G) * p.q.head_stride + cl * 8,
-                          p.q.fmt, q);
+                const int rr = 32 * wq + pass * RPP + lane / LPR;
+                const uint32_t r = rows.r0 + min((uint32_t)(sub * 128 + rr), rows.n - 1), tok = kv_div(r, p.group_magic);
+                const size_t at = (size_t)(seq.q0 + tok) * p.q.row_stride + (h * G + r - tok * G) * p.q.head_stride + cl * 8;
+                if constexpr (SPLIT) {
+                    kvf::cp_async16(place(rr), static_cast<const float *>(p.q.data) + at);
+                    kvf::cp_async16(place(rr) + S::DB * kBlk, static_cast<const float *>(p.q.data) + at + 4);
                 } else {
+                    kvf::cp_async16(place(rr), static_cast<const uint16_t *>(p.q.data) + at);
+                }
+            }
+            kvf::cp_commit();
+            kvf::cp_wait<0>();
+#pragma unroll 1
+            for (int pass = 0; pass < LPR; pass++) {
+                const int rr = 32 * wq + pass * RPP + lane / LPR;
+                const uint32_t dst = place(rr);
+                const float4 raw = lds4(dst);
+                float q[8];
+                if constexpr (SPLIT) {
+                    const float4 raw1 = lds4(dst + S::DB * kBlk);
+                    q[0] = raw.x; q[1] = raw.y; q[2] = raw.z; q[3] = raw.w;
+                    q[4] = raw1.x; q[5] = raw1.y; q[6] = raw1.z; q[7] = raw1.w;
+                } else {
+                    unpack16(make_uint4(__float_as_uint(raw.x), __float_as_uint(raw.y), __float_as_uint(raw.z),
+                                        __float_as_uint(raw.w)),
+                             p.q.fmt, q);
+                }
+                if ((uint32_t)(sub * 128 + rr) >= rows.n) {
 #pragma unroll
                     for (int i = 0; i < 8; i++) q[i] = 0.0f;
                 }
@@ -352,7 +373,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
                 const float sc = row_scale(amax);
                 // elements in the order the codes of a word unpack to
                 constexpr int o8[8] = {0, 1, 2, 3, 4, 5, 6, 7}, o4[8] = {0, 4, 1, 5, 2, 6, 3, 7};
-                uint32_t hi[4], lo[4];
+                uint32_t hi[4];
+                [[maybe_unused]] uint32_t lo[4];
                 float sum = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
@@ -369,7 +391,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
                 }
 #pragma unroll
                 for (int o = LPR / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                const uint32_t dst = qs + (cl >> 3) * kBlk + rr * 128 + (((cl & 7) ^ (rr & 7)) << 4);
                 sts4(dst, hi[0], hi[1], hi[2], hi[3]);
                 if constexpr (SPLIT) sts4(dst + S::DB * kBlk, lo[0], lo[1], lo[2], lo[3]);
                 if (cl == 0) {
@@ -391,7 +412,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
 #pragma unroll
         for (int k = 0; k < 4; k++) {
             const uint32_t in_tile = (uint32_t)(base_row + g + 8 * k);
-            pos[k] = in_tile < rows.n ? pos0 + (int)((rows.r0 + in_tile) / G) : -1;
+            pos[k] = in_tile < rows.n ? pos0 + (int)kv_div(rows.r0 + in_tile, p.group_magic) : -1;
             xs2[k] = pk(row_x[in_tile], row_x[in_tile]);
             qsum2[k] = pk(row_sum[in_tile], row_sum[in_tile]);
             // rows that see nothing start with a reference of their own: they never ask for one
@@ -593,48 +614,41 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
                     }
                 }
             };
-            auto load = [&](int q, uint32_t(&dst)[2][16]) {
-                tmem_ld_16x256_x4(scol + 32 * q, dst[0]);
-                tmem_ld_16x256_x4(scol + kHalf + 32 * q, dst[1]);
+            // A quarter of the tile at a time, rolled: the code of a tile has to stay in the
+            // instruction caches (four quarters unrolled, with the next one's loads ahead,
+            // was slower: 470 against 378 us a round of CTAs at 16384 tokens, and the more
+            // so the further the SMs are apart in their tiles).
+            auto quarter = [&](auto masked, auto tried, int q, unsigned on) -> unsigned {
+                uint32_t s[2][16], ph[2][8];
+                [[maybe_unused]] uint32_t pl[2][8];
+                f2 l_c[4];
+                [[maybe_unused]] f2 z_c[4];
+                tmem_ld_16x256_x4(scol + 32 * q, s[0]);
+                tmem_ld_16x256_x4(scol + kHalf + 32 * q, s[1]);
+                tmem_wait(s[0]);
+                tmem_wait(s[1]);
+                const float most = weigh(masked, q, s, ph, pl, l_c, z_c);
+                if constexpr (decltype(tried)::value) on &= __any_sync(0xffffffffu, most > fast_lim) ? 0u : 1u;
+                keep(on, q, ph, pl, l_c, z_c);
+                return on;
             };
+            // The old references are tried first; a weight is at most the sum of p times the
+            // largest scale, and from the first quarter where that says nothing on, the
+            // second loop takes over with new ones.
             auto tile = [&](auto masked) {
-                // Common path: the old references hold for the whole tile.  A weight is at
-                // most the sum of p times the largest scale; from the first quarter where
-                // that says nothing on, the second loop takes over.
                 int q = 0;
                 if (!__any_sync(0xffffffffu, unset)) {
-                    uint32_t s[2][2][16];
                     unsigned on = 1;
-                    load(0, s[0]);
-#pragma unroll
+#pragma unroll 1
                     for (int u = 0; u < 4; u++) {
-                        uint32_t ph[2][8];
-                        [[maybe_unused]] uint32_t pl[2][8];
-                        f2 l_c[4];
-                        [[maybe_unused]] f2 z_c[4];
-                        tmem_wait(s[u & 1][0]);
-                        tmem_wait(s[u & 1][1]);
-                        if (u < 3) load(u + 1, s[(u + 1) & 1]);
-                        const float most = weigh(masked, u, s[u & 1], ph, pl, l_c, z_c);
-                        on &= __any_sync(0xffffffffu, most > fast_lim) ? 0u : 1u;
-                        keep(on, u, ph, pl, l_c, z_c);
+                        on = quarter(masked, std::true_type{}, u, on);
                         q += (int)on;
                     }
                 }
                 if (q < 4) {
                     new_reference(q);
 #pragma unroll 1
-                    for (; q < 4; q++) {
-                        uint32_t s[2][16], ph[2][8];
-                        [[maybe_unused]] uint32_t pl[2][8];
-                        f2 l_c[4];
-                        [[maybe_unused]] f2 z_c[4];
-                        load(q, s);
-                        tmem_wait(s[0]);
-                        tmem_wait(s[1]);
-                        weigh(masked, q, s, ph, pl, l_c, z_c);
-                        keep(1u, q, ph, pl, l_c, z_c);
-                    }
+                    for (; q < 4; q++) quarter(masked, std::false_type{}, q, 1u);
                 }
             };
             if (whole) tile(std::false_type{});
@@ -670,14 +684,20 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
         ok = __all_sync(0xffffffffu, ok);
         if (ok) {
             tc_fence_after();
-            const uint32_t in_tile = (uint32_t)(base_row + lane), r = rows.r0 + in_tile;
+            const uint32_t in_tile = (uint32_t)(base_row + lane);
             const bool valid = in_tile < rows.n;
             const float l = row_x[in_tile], z = row_sum[in_tile];
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             const uint32_t tile_id = (b * p.cache.hkv + h) * p.row_tiles + rt;
             float *rec = p.nsplit > 1 ? p.part + kvf::few_record(tile_id, kRows, in_tile, p.nsplit, split) * (D + 2)
                                       : nullptr;
-            const size_t at = (size_t)(seq.q0 + r / G) * p.out.row_stride + (h * G + r % G) * p.out.head_stride;
+            // Finished rows go through the warp's quarter of its Q tile (every product has
+            // completed), 16-byte chunks XORed with the row, so that a row leaves in whole
+            // lines; parts of a split go out as they are.
+            constexpr int ES = SPLIT ? 4 : 2, ROWB = D * ES, CPR = ROWB / 16;  // bytes, chunks of a row
+            constexpr int SWZ = CPR < 8 ? CPR - 1 : 7;
+            const uint32_t stage = sbase + sub * S::Q_SUB + wq * (S::Q_SUB / 4);
+            static_assert(32 * ROWB <= S::Q_SUB / 4, "a warp's rows fit its quarter of Q");
 #pragma unroll 1
             for (int d0 = 0; d0 < D; d0 += 32) {
                 float o[32];
@@ -687,90 +707,98 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
 #pragma unroll
                     for (int j = 0; j < 32; j++) o[j] = 0.0f;
                 }
-                if (valid) {
 #pragma unroll
-                    for (int u = 0; u < 4; u++) {
-                        // positions of elements 0..7 within a unit of value codes
-                        constexpr int i8[8] = {0, 1, 2, 3, 4, 5, 6, 7}, i4[8] = {0, 2, 4, 6, 1, 3, 5, 7};
-                        float v[8];
+                for (int u = 0; u < 4; u++) {
+                    // positions of elements 0..7 within a unit of value codes
+                    constexpr int i8[8] = {0, 1, 2, 3, 4, 5, 6, 7}, i4[8] = {0, 2, 4, 6, 1, 3, 5, 7};
+                    float v[8];
 #pragma unroll
-                        for (int e = 0; e < 8; e++) v[e] = (o[8 * u + (BV == 8 ? i8[e] : i4[e])] + z) * unit;
-                        if (rec) {
+                    for (int e = 0; e < 8; e++) v[e] = (o[8 * u + (BV == 8 ? i8[e] : i4[e])] + z) * unit;
+                    if (rec) {
+                        if (valid) {
 #pragma unroll
                             for (int e = 0; e < 8; e += 2)
                                 *reinterpret_cast<float2 *>(rec + d0 + 8 * u + e) = make_float2(v[e], v[e + 1]);
-                        } else {
+                        }
+                    } else {
 #pragma unroll
-                            for (int e = 0; e < 8; e++) v[e] *= inv;
-                            store8(p.out.data, at + d0 + 8 * u, p.out.fmt, v);
+                        for (int e = 0; e < 8; e++) v[e] *= inv;
+                        const uint32_t row = stage + lane * ROWB;
+                        const int ch = (d0 + 8 * u) * ES / 16;
+                        if constexpr (SPLIT) {
+                            sts4(row + ((ch ^ (lane & SWZ)) << 4), __float_as_uint(v[0]), __float_as_uint(v[1]),
+                                 __float_as_uint(v[2]), __float_as_uint(v[3]));
+                            sts4(row + (((ch + 1) ^ (lane & SWZ)) << 4), __float_as_uint(v[4]), __float_as_uint(v[5]),
+                                 __float_as_uint(v[6]), __float_as_uint(v[7]));
+                        } else {
+                            sts4(row + ((ch ^ (lane & SWZ)) << 4), pack16(v[0], v[1], p.out.fmt), pack16(v[2], v[3], p.out.fmt),
+                                 pack16(v[4], v[5], p.out.fmt), pack16(v[6], v[7], p.out.fmt));
                         }
                     }
+                }
+            }
+            if (!rec) {
+                __syncwarp();
+                constexpr int RPI = 32 / CPR;  // rows of one store
+#pragma unroll 4
+                for (int it = 0; it < CPR; it++) {
+                    const int rr = it * RPI + lane / CPR, ch = lane % CPR;
+                    const float4 v = lds4(stage + rr * ROWB + ((ch ^ (rr & SWZ)) << 4));
+                    const uint32_t tile_row = (uint32_t)(base_row + rr), gr = rows.r0 + tile_row;
+                    const uint32_t tok = kv_div(gr, p.group_magic);
+                    if (tile_row < rows.n)
+                        *reinterpret_cast<float4 *>(static_cast<uint8_t *>(p.out.data) +
+                                                    ((size_t)(seq.q0 + tok) * p.out.row_stride +
+                                                     (h * G + gr - tok * G) * p.out.head_stride) * ES + ch * 16) = v;
                 }
             }
             if (rec && valid) *reinterpret_cast<float2 *>(rec + D) = make_float2(l == 0.0f ? -INFINITY : row_ref[in_tile], l);
         }
     } else if (warp < 12) {
         // ================= producers: codes to f16 operands =================
-        regs_dec<kRegsProducer>();
-        const int pt = threadIdx.x - 256;
+        set_regs<kRegsProducer>();
+        const bool keys = warp < 10;
+        const int pw = warp & 1;
         const uint32_t *table = p.batch.table + (size_t)b * p.batch.stride;
         const uint32_t mask = (1u << p.cache.shift) - 1u;
-        // lane l < 8: the page of run l (16 tokens) of tile i; ~0: nothing to read there
-        auto run_pages = [&](uint32_t i) -> uint32_t {
+        // Lane l < 8: the page of run l (16 tokens) of tile i, ~0 where nothing of it is
+        // read.  (Loaded two tiles ahead; looked at by page_ok.)
+        auto load_pages = [&](uint32_t i) -> uint32_t {
             if (i >= n || lane >= kTok / 16) return ~0u;
             const uint32_t j = tile_token(i) + 16 * lane;
-            if (!kv_needed(range, j, j + 16)) return ~0u;
-            const uint32_t page = __ldg(table + (j >> p.cache.shift));
+            return kv_needed(range, j, j + 16) ? __ldg(table + (j >> p.cache.shift)) : ~0u;
+        };
+        auto page_ok = [&](uint32_t page, uint32_t i) -> uint32_t {
             if (page < p.cache.num_pages) return page;
-            fault = KV_FAULT_PAGE;
+            if (i < n && lane < kTok / 16) {
+                const uint32_t j = tile_token(i) + 16 * lane;
+                if (kv_needed(range, j, j + 16)) fault = KV_FAULT_PAGE;
+            }
             return ~0u;
         };
         auto slot_of = [&](uint32_t page, uint32_t j) {
             return (((size_t)page * p.cache.hkv + h) << p.cache.shift) + (j & mask);
         };
-        uint4 kr[Chunks<D, BK>::N], vr[Chunks<D, BV>::N];
-        float rs[4];
         // A thread's chunks of 16 bytes: LC lanes a row, so that the eight lanes of
         // a store phase write eight different 16-byte columns of the swizzled rows
+        // Lane l < 8 finds run l; runs without a page read page 0 (their weights are
+        // zero whatever the codes), so that no load waits for a branch.
         auto load_codes = [&](auto bits_c, uint4 *dst, const uint8_t *codes, uint32_t pages, uint32_t i) {
             using C = Chunks<D, decltype(bits_c)::value>;
-            const uint32_t j0 = tile_token(i);
+            const uint64_t run = reinterpret_cast<uint64_t>(codes) +
+                                 slot_of(pages == ~0u ? 0u : pages, tile_token(i) + 16 * lane) * (C::CPR * 16);
+            uint64_t from = 0;
 #pragma unroll
             for (int it = 0; it < C::N; it++) {
-                const uint32_t row = C::row(it, warp - 8, lane), col = C::col(it, lane);
-                const uint32_t page = __shfl_sync(0xffffffffu, pages, row >> 4);
-                dst[it] = make_uint4(0u, 0u, 0u, 0u);
-                if (page != ~0u)
-                    dst[it] = ld_stream(
-                        reinterpret_cast<const uint4 *>(codes + slot_of(page, j0 + row) * (C::N * 16) + col * 16));
-            }
-        };
-        auto load_scales = [&](uint32_t pages, uint32_t i) {
-            const uint32_t j = tile_token(i) + pt;
-            const uint32_t page = __shfl_sync(0xffffffffu, pages, pt >> 4);
-            rs[0] = rs[1] = rs[2] = rs[3] = 0.0f;
-            if (page != ~0u && kv_needed(range, j, j + 1)) {
-                const size_t slot = slot_of(page, j);
-                if constexpr (BK == 8) {
-                    rs[0] = __ldg(p.cache.scales[0] + slot);
-                } else {
-                    const float2 v = __ldg(reinterpret_cast<const float2 *>(p.cache.scales[0]) + slot);
-                    rs[0] = v.x;
-                    rs[1] = v.y;
-                }
-                if constexpr (BV == 8) {
-                    rs[2] = __ldg(p.cache.scales[1] + slot);
-                } else {
-                    const float2 v = __ldg(reinterpret_cast<const float2 *>(p.cache.scales[1]) + slot);
-                    rs[2] = v.x;
-                    rs[3] = v.y;
-                }
+                const uint32_t row = C::row(it, pw, lane), col = C::col(it, lane);
+                if (it % C::PER == 0) from = __shfl_sync(0xffffffffu, run, row >> 4) + (row & 15) * (C::CPR * 16);
+                dst[it] = ld_stream(reinterpret_cast<const uint4 *>(from + col * 16));
             }
         };
         auto store_codes = [&](auto bits_c, const uint4 *src, uint32_t base) {
             constexpr int BITS = decltype(bits_c)::value;
             using C = Chunks<D, BITS>;
-            const uint32_t row0 = C::row(0, warp - 8, lane), at = base + row0 * 128;
+            const uint32_t row0 = C::row(0, pw, lane), at = base + row0 * 128;
             const uint32_t c16 = ((uint32_t)(lane % C::LC) * (BITS == 8 ? 2 : 4) ^ (row0 & 7)) << 4;
 #pragma unroll
             for (int it = 0; it < C::N; it++) {
@@ -792,86 +820,134 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
                 }
             }
         };
-        const std::integral_constant<int, BK> kbits{};
-        const std::integral_constant<int, BV> vbits{};
-        // power of two on the values' scales and zeros (0: none of them seen so far
-        // but zero), the same in all four warps, and its reciprocal
-        float lift = 0.0f, unit = 1.0f;
-        uint32_t cur = run_pages(0);
-        if (n > 0) {
-            load_codes(kbits, kr, p.cache.codes[0], cur, 0);
-            load_scales(cur, 0);
-        }
         bool ok = true;
-        for (uint32_t i = 0; i < n; i++) {
-            const uint32_t st = i % ST, ph = (i / ST) & 1;
-            load_codes(vbits, vr, p.cache.codes[1], cur, i);
-            const uint32_t nxt = run_pages(i + 1);
-            ok = __all_sync(0xffffffffu, wait_or_fault(&kempty[st], ph ^ 1, &abort_s, p.fault));
-            if (!ok) break;
-            store_codes(kbits, kr, sbase + S::K0 + st * S::KV);
-            const uint32_t sl = sbase + S::SC + (i % kScaleSlots) * Slot::BYTES;
-            if (lift == 0.0f) {
-                // every warp looks at the whole tile: no wait between warps
-                float mag = 0.0f;
+        uint32_t next = load_pages(0);
+        if (keys) {
+            const std::integral_constant<int, BK> kbits{};
+            // Scales and zeros of tokens pt and pt + 64: key, value
+            const int pt = 32 * pw + lane;
+            uint4 kr[Chunks<D, BK>::N];
+            float rs[2][4];
+            auto load_scales = [&](uint32_t pages, uint32_t i) {
 #pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    const uint32_t j = tile_token(i) + 32 * q + lane;
-                    const uint32_t page = __shfl_sync(0xffffffffu, cur, (32 * q + lane) >> 4);
+                for (int t = 0; t < 2; t++) {
+                    const uint32_t j = tile_token(i) + pt + 64 * t;
+                    const uint32_t page = __shfl_sync(0xffffffffu, pages, (pt + 64 * t) >> 4);
+                    rs[t][0] = rs[t][1] = rs[t][2] = rs[t][3] = 0.0f;
                     if (page == ~0u || !kv_needed(range, j, j + 1)) continue;
-                    if constexpr (BV == 8) {
-                        mag = fmaxf(mag, __ldg(p.cache.scales[1] + slot_of(page, j)));
+                    const size_t slot = slot_of(page, j);
+                    if constexpr (BK == 8) {
+                        rs[t][0] = __ldg(p.cache.scales[0] + slot);
                     } else {
-                        const float2 v = __ldg(reinterpret_cast<const float2 *>(p.cache.scales[1]) + slot_of(page, j));
-                        mag = fmaxf(mag, fmaxf(v.x, fabsf(v.y)));
+                        const float2 v = __ldg(reinterpret_cast<const float2 *>(p.cache.scales[0]) + slot);
+                        rs[t][0] = v.x;
+                        rs[t][1] = v.y;
+                    }
+                    if constexpr (BV == 8) {
+                        rs[t][2] = __ldg(p.cache.scales[1] + slot);
+                    } else {
+                        const float2 v = __ldg(reinterpret_cast<const float2 *>(p.cache.scales[1]) + slot);
+                        rs[t][2] = v.x;
+                        rs[t][3] = v.y;
                     }
                 }
-                mag = warp_max(mag);
-                if (mag > 0.0f) {
-                    lift = __int_as_float((127 + kvf::near_one(mag)) << 23);
-                    unit = __int_as_float((127 - kvf::near_one(mag)) << 23);
+            };
+            // power of two on the values' scales and zeros (0: none of them seen so far
+            // but zero), the same in both warps, and its reciprocal
+            float lift = 0.0f, unit = 1.0f;
+            uint32_t cur = page_ok(next, 0);
+            if (n > 0) {
+                load_codes(kbits, kr, p.cache.codes[0], cur, 0);
+                load_scales(cur, 0);
+            }
+            next = load_pages(1);
+            for (uint32_t i = 0; i < n; i++) {
+                const uint32_t st = i % ST, ph = (i / ST) & 1;
+                ok = __all_sync(0xffffffffu, wait_or_fault(&kempty[st], ph ^ 1, &abort_s, p.fault));
+                if (!ok) break;
+                store_codes(kbits, kr, sbase + S::K0 + st * S::KV);
+                const uint32_t sl = sbase + S::SC + (i % kScaleSlots) * Slot::BYTES;
+                if (lift == 0.0f) {
+                    // both warps look at the whole tile: no wait between them
+                    float mag = 0.0f;
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        const uint32_t j = tile_token(i) + 32 * q + lane;
+                        const uint32_t page = __shfl_sync(0xffffffffu, cur, (32 * q + lane) >> 4);
+                        if (page == ~0u || !kv_needed(range, j, j + 1)) continue;
+                        if constexpr (BV == 8) {
+                            mag = fmaxf(mag, __ldg(p.cache.scales[1] + slot_of(page, j)));
+                        } else {
+                            const float2 v = __ldg(reinterpret_cast<const float2 *>(p.cache.scales[1]) + slot_of(page, j));
+                            mag = fmaxf(mag, fmaxf(v.x, fabsf(v.y)));
+                        }
+                    }
+                    mag = warp_max(mag);
+                    if (mag > 0.0f) {
+                        lift = __int_as_float((127 + kvf::near_one(mag)) << 23);
+                        unit = __int_as_float((127 - kvf::near_one(mag)) << 23);
+                    }
                 }
+#pragma unroll
+                for (int t = 0; t < 2; t++) {
+                    const uint32_t at = sl + 4 * (pt + 64 * t);
+                    float sv = rs[t][2] * lift, zv = rs[t][3] * lift;
+                    if (!(fabsf(sv) <= 3.4e38f && fabsf(zv) <= 3.4e38f)) {
+                        // not a number: the score says so to the rows that see the token,
+                        // the others multiply its value by zero
+                        rs[t][0] = kv_nan();
+                        sv = zv = 0.0f;
+                    }
+                    sts1(at + Slot::SK, rs[t][0]);
+                    sts1(at + Slot::SV, sv);
+                    sts1(at + Slot::LV, lg2(fmaxf(sv, fabsf(zv))));
+                    if constexpr (BK == 4) sts1(at + Slot::ZK, rs[t][1]);
+                    if constexpr (BV == 4) sts1(at + Slot::ZV, zv);
+                    const float sm = warp_max(sv), zm = BV == 4 ? warp_max(fabsf(zv)) : 0.0f;
+                    if (lane == 0) {
+                        sts1(sl + Slot::SMAX + 4 * (pw + 2 * t), sm);
+                        sts1(sl + Slot::ZMAX + 4 * (pw + 2 * t), zm);
+                    }
+                }
+                if (pt == 0) sts1(sl + Slot::UNIT, unit);
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&scfull[i % kScaleSlots]);
+                    mbar_arrive(&kfull[st]);
+                }
+                cur = page_ok(next, i + 1);
+                if (i + 1 < n) {
+                    load_codes(kbits, kr, p.cache.codes[0], cur, i + 1);
+                    load_scales(cur, i + 1);
+                }
+                next = load_pages(i + 2);
             }
-            rs[2] *= lift;
-            rs[3] *= lift;
-            if (!(fabsf(rs[2]) <= 3.4e38f && fabsf(rs[3]) <= 3.4e38f)) {
-                // not a number: the score says so to the rows that see the token, the
-                // others multiply its value by zero
-                rs[0] = kv_nan();
-                rs[2] = rs[3] = 0.0f;
+            if (fault) kv_report(p.fault, fault);
+        } else {
+            const std::integral_constant<int, BV> vbits{};
+            uint4 vr[Chunks<D, BV>::N];
+            if (n > 0) load_codes(vbits, vr, p.cache.codes[1], page_ok(next, 0), 0);
+            next = load_pages(1);
+            for (uint32_t i = 0; i < n; i++) {
+                const uint32_t st = i % ST, ph = (i / ST) & 1;
+                ok = __all_sync(0xffffffffu, wait_or_fault(&vempty[st], ph ^ 1, &abort_s, p.fault));
+                if (!ok) break;
+                store_codes(vbits, vr, sbase + S::V0 + st * S::KV);
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&vfull[st]);
+                const uint32_t cur = page_ok(next, i + 1);
+                if (i + 1 < n) load_codes(vbits, vr, p.cache.codes[1], cur, i + 1);
+                next = load_pages(i + 2);
             }
-            sts1(sl + Slot::SK + 4 * pt, rs[0]);
-            sts1(sl + Slot::SV + 4 * pt, rs[2]);
-            sts1(sl + Slot::LV + 4 * pt, lg2(fmaxf(rs[2], fabsf(rs[3]))));
-            if constexpr (BK == 4) sts1(sl + Slot::ZK + 4 * pt, rs[1]);
-            if constexpr (BV == 4) sts1(sl + Slot::ZV + 4 * pt, rs[3]);
-            const float sm = warp_max(rs[2]), zm = BV == 4 ? warp_max(fabsf(rs[3])) : 0.0f;
-            if (lane == 0) {
-                sts1(sl + Slot::SMAX + 4 * (warp - 8), sm);
-                sts1(sl + Slot::ZMAX + 4 * (warp - 8), zm);
-            }
-            if (pt == 0) sts1(sl + Slot::UNIT, unit);
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(&scfull[i % kScaleSlots]);
-                mbar_arrive(&kfull[st]);
-            }
-            if (i + 1 < n) {
-                load_codes(kbits, kr, p.cache.codes[0], nxt, i + 1);
-                load_scales(nxt, i + 1);
-            }
-            ok = __all_sync(0xffffffffu, wait_or_fault(&vempty[st], ph ^ 1, &abort_s, p.fault));
-            if (!ok) break;
-            store_codes(vbits, vr, sbase + S::V0 + st * S::KV);
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&vfull[st]);
-            cur = nxt;
         }
-        if (fault) kv_report(p.fault, fault);
-    } else if (regs_dec<kRegsIssue>(); warp == 12) {
+    } else if (set_regs<kRegsIssue>(); warp == 12) {
         // ================= MMA issue (whole warp, elected lane) =================
+        // One warp for both row tiles, in turn: each tile's products run while the
+        // other's softmax does (with a warp each, the two fell into step and the
+        // tensor pipe waited: 5.2 against 4.8 us a key tile).  The products run in
+        // the order of issue: P V reads P before the next S is written over it.
         constexpr uint32_t id_s = idesc_f16(kTok, false), id_o = idesc_f16(D, true);
         const uint32_t q0 = sbase, k0 = sbase + S::K0, v0 = sbase + S::V0;
         unsigned pc[2] = {0, 0};  // products of P done so far, per row tile

@@ -12,6 +12,21 @@ constexpr int kFmtF32 = 0, kFmtF16 = 1, kFmtBf16 = 28;  // NEXUS_FMT_*
 
 __device__ __forceinline__ float kv_nan() { return __int_as_float(0x7fffffff); }
 
+// Eight f16 or bf16 elements of 16 bytes.
+__device__ __forceinline__ void unpack16(const uint4 &a, int fmt, float (&v)[8]) {
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if (fmt == kFmtBf16) {
+            v[2 * i] = __uint_as_float(w[i] << 16);
+            v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        } else {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+            v[2 * i] = f.x;
+            v[2 * i + 1] = f.y;
+        }
+    }
+}
 // Eight consecutive elements (16-byte aligned) as f32.
 __device__ __forceinline__ void load8(const void *base, size_t elem, int fmt, float (&v)[8]) {
     if (fmt == kFmtF32) {
@@ -20,19 +35,7 @@ __device__ __forceinline__ void load8(const void *base, size_t elem, int fmt, fl
         v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
         v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
     } else {
-        const uint4 a = __ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(base) + elem));
-        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            if (fmt == kFmtBf16) {
-                v[2 * i] = __uint_as_float(w[i] << 16);
-                v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-            } else {
-                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
-                v[2 * i] = f.x;
-                v[2 * i + 1] = f.y;
-            }
-        }
+        unpack16(__ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(base) + elem)), fmt, v);
     }
 }
 __device__ __forceinline__ uint32_t pack16(float a, float b, int fmt) {

@@ -99,6 +99,14 @@ NX_HD KvTiles kv_tiles(const KvRange &r, uint32_t T) {
 }
 NX_HD uint32_t kv_tile_at(const KvTiles &t, uint32_t i) { return i < t.sink_tiles ? i : t.first + (i - t.sink_tiles); }
 
+// r / G by multiplication: exact for r < 2^32 / G with magic = ceil(2^32 / G).
+// A row's number is below 2^24 in the chunk kernel (its grid's limit of 65535
+// tiles of 256 rows) and G at most 128.
+NX_HD uint32_t kv_div_magic(uint32_t G) { return G == 1 ? 0u : (uint32_t)(((1ull << 32) + G - 1) / G); }
+NX_HD uint32_t kv_div(uint32_t r, uint32_t magic) {
+    return magic == 0 ? r : (uint32_t)(((uint64_t)r * magic) >> 32);
+}
+
 // Tile rt of R rows of a sequence's (token, head of the group) rows: n rows
 // from r0 on, of the tokens at positions first .. last.  Sequences of more
 // than `limit` rows are another kernel's (n = 0).

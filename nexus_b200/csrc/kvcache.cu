@@ -278,6 +278,7 @@ extern "C" int nexus_cuda_kv_attention(nexus_cuda_backend *b, const nexus_kv_cac
     p.out = rows_view(out);
     p.hq = (int)q->heads;
     p.group = (int)(q->heads / cache->kv_heads);
+    p.group_magic = kv_div_magic((uint32_t)p.group);
     p.scale_log2 = (scale != 0.0f ? scale : 1.0f / sqrtf((float)cache->head_dim)) * 1.4426950408889634f;
     p.window = window;
     p.sinks = sinks;

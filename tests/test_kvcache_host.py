@@ -189,6 +189,12 @@ int main() {
             if (ordered && b == (uint32_t)n) CHECK(n == 0 || row >= q[n]);
         }
     }
+    // division by the group for every row number the chunk kernel has
+    for (uint32_t G = 1; G <= 128; G++) {
+        const uint32_t m = kv_div_magic(G);
+        for (uint32_t r = 0; r < 70000; r++) CHECK(kv_div(r, m) == r / G);
+        for (uint32_t r = 65535u * 256u; r > 65535u * 256u - 70000u; r--) CHECK(kv_div(r, m) == r / G);
+    }
     // row tiles cover every (token, head) row once, positions in step
     for (uint32_t G : {1u, 3u, 4u, 5u, 8u, 40u, 128u}) for (uint32_t nq : {0u, 1u, 2u, 33u}) for (uint32_t R : {8u, 16u, 128u}) {
         const KvSeqView s = {7, nq, 20};
