@@ -46,6 +46,7 @@ struct KvAttnParams {
     // split over the context
     uint32_t nsplit, tiles_per_split;
     float *part;               // records of unfinished softmaxes (nsplit > 1)
+    float *sums;               // chunk kernel, f32 queries: a CTA's output sums
     // sequences of at most rows_limit (token, head) rows per KV head are the
     // few-row kernel's, the others the chunk kernel's
     uint32_t rows_limit;
@@ -58,6 +59,7 @@ struct KvAttnParams {
 constexpr uint32_t kKvFewRows = 16;
 constexpr uint32_t kKvChunkRows = 256;   // rows of a chunk-kernel CTA
 constexpr uint32_t kKvChunkTile = 128;   // tokens of its key tile
+constexpr uint32_t kKvFlushTiles = 2;    // f32 queries: key tiles summed in tensor memory
 constexpr uint32_t kKvFewTile = 16;      // tokens of one warp's tile
 constexpr uint32_t kKvFewWarps = 4;
 constexpr uint32_t kKvSms = 148;

@@ -28,6 +28,10 @@
 // S and O of both tiles fill tensor memory; P overwrites S in place.  While the
 // softmax of one tile runs, the tensor pipe works for the other.  Keys come in
 // by registers rather than TMA because they must be unpacked on the way.
+// The tensor cores round each sum toward zero, an error that grows with the number
+// of products summed in place (4.5e-5 of the output after 40000 tokens).  For f32
+// queries the output is therefore taken out of tensor memory every kFlush tiles
+// and added, correctly rounded, to sums in the caller's workspace.
 // Every wait is bounded (as in kernels_gemm.cuh).
 #pragma once
 #include <type_traits>
@@ -55,6 +59,7 @@ constexpr float kUp = 4.0f;             // a new reference puts the largest weig
 constexpr float kMaxWeight = 65504.0f;  // and it is moved when a weight would leave f16
 constexpr float kMaxProb = 60.0f;       // log2 of the largest p where values are zero
 constexpr int kScaleSlots = 4;
+constexpr int kFlush = kKvFlushTiles;
 
 // What the softmax needs of a key tile, by token; byte offsets in shared memory.
 struct Slot {
@@ -420,6 +425,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
             nref2[k] = pk(0.0f, 0.0f);
             l2[k] = z2[k] = pk(0.0f, 0.0f);  // sums of p and p zv of this thread's columns
         }
+        // f32 queries: this thread's sums in the workspace (32 lanes of one element next to
+        // each other), what they are to be multiplied by to be in the references' terms,
+        // and whether there are any
+        [[maybe_unused]] float *sums = nullptr;
+        [[maybe_unused]] float sum_f[4] = {1.0f, 1.0f, 1.0f, 1.0f};
+        [[maybe_unused]] bool summed = false;
+        if constexpr (SPLIT)
+            sums = p.sums + ((((size_t)b * p.cache.hkv + h) * p.row_tiles + rt) * p.nsplit + split) * (kRows * D) +
+                   warp * (32 * D) + lane;
         bool unset = true;  // some reference may not be set yet
         float unit = 1.0f;
         const int first = sub ? first1 : rows.first, last = sub ? rows.last : last0;
@@ -427,6 +441,35 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
         constexpr uint32_t kHalf = 16u << 16;  // the second half of the warp's lanes
         unsigned cnt = 0;
         bool ok = true;
+        // The output in tensor memory (complete) and the sums: to_sums, into the sums;
+        // otherwise their total back into tensor memory.
+        [[maybe_unused]] auto flush = [&](bool to_sums) {
+#pragma unroll 1
+            for (int q = 0; q < D / 32; q++) {
+#pragma unroll
+                for (int hh = 0; hh < 2; hh++) {
+                    uint32_t o[16];
+                    float *at = sums + (q * 2 + hh) * 512;
+                    tmem_ld_16x256_x4(ocol + hh * kHalf + 32 * q, o);
+                    tmem_wait(o);
+                    if (summed) {
+#pragma unroll
+                        for (int j = 0; j < 16; j++)
+                            o[j] = __float_as_uint(fmaf(__ldcg(at + 32 * j), sum_f[2 * hh + (j >> 1 & 1)], __uint_as_float(o[j])));
+                    }
+                    if (to_sums) {
+#pragma unroll
+                        for (int j = 0; j < 16; j++) __stcg(at + 32 * j, __uint_as_float(o[j]));
+                    } else {
+                        tmem_st_16x256_x4(ocol + hh * kHalf + 32 * q, o);
+                    }
+                }
+            }
+            if (!to_sums) tmem_wait_st();
+            summed = true;
+#pragma unroll
+            for (int k = 0; k < 4; k++) sum_f[k] = 1.0f;
+        };
         for (uint32_t i = 0; i < n; i++) {
             if (!active(sub, i)) continue;
             const int j0 = (int)tile_token(i);
@@ -436,6 +479,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tc_fence_after();
+            if constexpr (SPLIT) {
+                if (cnt > 0 && cnt % kFlush == 0) flush(true);  // (the products before S have completed)
+            }
             const bool whole = j0 + kTok - 1 <= first &&
                                (p.window == 0 || j0 > last - (int)p.window || j0 + kTok <= (int)p.sinks);
             unit = lds1(sl + Slot::UNIT);
@@ -508,6 +554,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
                     nref2[k] = next == -INFINITY ? pk(0.0f, 0.0f) : pk(-next, -next);
                     unset |= next == -INFINITY;
                     moved |= f[k] != 1.0f;
+                    if constexpr (SPLIT) sum_f[k] *= f[k];
                     l2[k] = mul2(l2[k], pk(f[k], f[k]));
                     z2[k] = mul2(z2[k], pk(f[k], f[k]));
                 }
@@ -684,6 +731,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
         ok = __all_sync(0xffffffffu, ok);
         if (ok) {
             tc_fence_after();
+            if constexpr (SPLIT) {
+                if (summed) flush(false);
+            }
             const uint32_t in_tile = (uint32_t)(base_row + lane);
             const bool valid = in_tile < rows.n;
             const float l = row_x[in_tile], z = row_sum[in_tile];
@@ -973,7 +1023,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
             for (int ks = 0; ks < kTok / 16; ks++) {  // (two products a step for f32 queries)
                 const uint64_t bd = desc_sw128(v0 + st * S::KV + ks * 2048, kBlk);
                 const uint32_t a = tmem + kSCol + 128 * sub + (SPLIT ? 16 * ks : 8 * ks);
-                umma_f16_ts_w(tmem + kOCol + D * sub, a, bd, id_o, pc[sub] != 0 || ks != 0);
+                umma_f16_ts_w(tmem + kOCol + D * sub, a, bd, id_o, (SPLIT ? pc[sub] % kFlush : pc[sub]) != 0 || ks != 0);
                 if constexpr (SPLIT) umma_f16_ts_w(tmem + kOCol + D * sub, a + 8, bd, id_o, 1);
             }
         };

@@ -129,6 +129,7 @@ struct AttnPlan {
     uint32_t rows_limit;  // sequences of more rows than this go to the chunk kernel
     bool few, chunk;
     Split f, c;
+    size_t sums;  // chunk kernel's sums of f32 queries
     size_t bytes;
 };
 
@@ -175,8 +176,10 @@ const char *attn_plan(const nexus_kv_cache *c, const nexus_kv_batch *t, const ne
         if (row_tiles * pl->c.nsplit > 65535) return "kv attention: too many rows per sequence for one call";
         pl->c.row_tiles = (uint32_t)row_tiles;
         pl->c.bytes = part_bytes(pl->c, ctas, c->head_dim);
+        if (q->format == NEXUS_FMT_F32 && per > kKvFlushTiles)
+            pl->sums = (size_t)ctas * pl->c.nsplit * kKvChunkRows * c->head_dim * sizeof(float);
     }
-    pl->bytes = pl->f.bytes + pl->c.bytes;
+    pl->bytes = pl->f.bytes + pl->c.bytes + pl->sums;
     return nullptr;
 }
 
@@ -293,7 +296,9 @@ extern "C" int nexus_cuda_kv_attention(nexus_cuda_backend *b, const nexus_kv_cac
         p.tiles_per_split = s.tiles_per_split;
         p.tile_rows = s.tile_rows;
         p.row_tiles = s.row_tiles;
-        p.part = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + (chunk ? pl.f.bytes : 0));
+        uint8_t *ws = static_cast<uint8_t *>(workspace);
+        p.part = reinterpret_cast<float *>(ws + (chunk ? pl.f.bytes : 0));
+        p.sums = reinterpret_cast<float *>(ws + pl.f.bytes + pl.c.bytes);
         if (r == cudaSuccess) r = chunk ? launch_kv_attn_chunk(p, st) : launch_kv_attn_few(p, st);
         if (r == cudaSuccess && p.nsplit > 1) r = launch_kv_merge(p, st);
     }

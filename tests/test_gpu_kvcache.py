@@ -415,6 +415,32 @@ def test_same_call_same_bits(backend, nb):
     cache.status()
 
 
+@pytest.mark.parametrize("dim,bits", [(128, (8, 8)), (64, (8, 4)), (32, (4, 8))])
+@pytest.mark.parametrize("new", [1, 40, 300])
+def test_f32_stays_exact_over_long_contexts(backend, nb, new, dim, bits):
+    """Sums over 20000 tokens whose values share a sign: an accumulator that rounds one way
+    loses 3e-5 here.  2e-6: two key tiles are 32 products rounded one way, half a step of
+    2^-23 each at most, of a sum that grows to its end (32 * 2^-24 / 2 = 1e-6), and S as much."""
+    lens = [(new, 20011)] + [(1, 20011)] * 40
+    batch, pages, rows = make_batch(nb, lens[:1], 64)
+    table = batch.page_table.expand(41, -1).contiguous()
+    starts = [0] + [new + i for i in range(41)]
+    batch = nb.KvBatch(torch.tensor(starts, dtype=torch.int32, device=DEV),
+                       torch.full((41,), 20011, dtype=torch.int32, device=DEV), table, new, 20011)
+    cache = nb.PagedKvCache.empty(backend, pages, 4, dim, 64, bits)
+    fill_random(cache, 50)
+    if bits[1] == 8:
+        cache.v_codes.copy_(cache.v_codes // 4 + 160)
+    else:
+        cache.v_scales[..., 1].abs_().add_(2.0)
+    q = torch.randn((new + 40, 8, dim), generator=gen(51), device=DEV)
+    out = cache.attention(batch, q)
+    cache.status()
+    for rows, ls in ((slice(0, new), [(new, 20011)]), (slice(new, new + 1), [(1, 20011)])):
+        ref = R.attention(q[rows], cache, ls, table)[0]
+        assert float((out[rows].double() - ref).norm() / ref.norm()) < 2e-6
+
+
 # ---------------------------------------------------------------- used together
 
 @pytest.mark.parametrize("bits", [(8, 8), (4, 4)])
