@@ -52,6 +52,7 @@ struct KvAttnParams {
     uint32_t rows_limit;
     uint32_t tile_rows, row_tiles;  // rows of a tile (8, 16; chunk 256), tiles a sequence may have
     int chunk;
+    int cluster;               // few-row kernel: the splits of a row tile are a cluster
 };
 
 // Rows of one KV head (new tokens x query heads of its group) of a sequence
@@ -63,6 +64,7 @@ constexpr uint32_t kKvFlushTiles = 2;    // f32 queries: key tiles summed in ten
 constexpr uint32_t kKvFewTile = 16;      // tokens of one warp's tile
 constexpr uint32_t kKvFewWarps = 4;
 constexpr uint32_t kKvSms = 148;
+constexpr uint32_t kKvCluster = 8;       // most splits that join as a cluster (the portable size)
 
 cudaError_t launch_kv_attn_few(const KvAttnParams &p, cudaStream_t st);
 cudaError_t launch_kv_attn_chunk(const KvAttnParams &p, cudaStream_t st);

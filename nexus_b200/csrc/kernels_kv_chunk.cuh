@@ -83,53 +83,6 @@ struct Smem {
     static constexpr int TOTAL = NEED > 120 * 1024 ? NEED : 120 * 1024;
 };
 
-// ---- packed pairs of f32 (two results an instruction) ----
-typedef unsigned long long f2;
-__device__ __forceinline__ f2 pk(float a, float b) {
-    f2 r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ void upk(f2 v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
-    f2 r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ f2 add2(f2 a, f2 b) {
-    f2 r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
-    f2 r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-
-__device__ __forceinline__ float4 lds4(uint32_t a) {
-    float4 v;
-    asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a));
-    return v;
-}
-__device__ __forceinline__ f2 lds2(uint32_t a) {
-    f2 v;
-    asm volatile("ld.shared.b64 %0, [%1];" : "=l"(v) : "r"(a));
-    return v;
-}
-__device__ __forceinline__ float lds1(uint32_t a) {
-    float v;
-    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a));
-    return v;
-}
-__device__ __forceinline__ void sts1(uint32_t a, float v) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory"); }
-__device__ __forceinline__ void sts4(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
-    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
-}
-__device__ __forceinline__ float max4(float4 v) { return fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)); }
-// the first n of 32 bits, any n
-__device__ __forceinline__ uint32_t first_bits(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
-
 // Tensor memory, 32 lanes of a warp as rows g, g + 8 (first half) and g + 16,
 // g + 24 (second), g = lane / 4, c = lane % 4.  Loads are complete after
 // tmem_wait; `r` is tied to it so that nothing reads it before.
@@ -726,6 +679,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
             }
         }
         __syncwarp();
+        pdl_launch_dependents();
         // ---- output ----
         if (ok) ok = wait_or_fault(&odone, 0, &abort_s, p.fault);
         ok = __all_sync(0xffffffffu, ok);

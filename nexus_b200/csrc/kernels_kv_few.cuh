@@ -25,23 +25,35 @@
 //    where the 128-row tcgen05 tile would be empty but for 4 of 128, and both
 //    operands are unpacked in registers, which tcgen05 could not read.
 //  - A warp owns 16-token tiles (one page holds a tile whole); their codes and
-//    scales come by cp.async into a ring of four slots of its own, so three
-//    tiles a warp are in flight and no barrier is in the loop.
-//  - The context is split over CTAs; kv_merge_few joins the parts in order.
+//    scales come by cp.async into a ring of three slots of its own, so two tiles a
+//    warp are in flight and no barrier is in the loop.
+//  - The context is split over CTAs.  Up to eight parts are a cluster, which joins
+//    them through distributed shared memory (parts beyond a sequence's end leave at
+//    once); more go to the workspace and k_kv_merge joins them.  Either way in order.
 #pragma once
+#include <type_traits>
+
 #include "kv_math.cuh"
 
 namespace nx {
 namespace kvf {
 
 constexpr int kWarps = kKvFewWarps;
-constexpr int kStages = 4;
-constexpr float kUp = 10.0f;       // log2 of the largest weight under a new reference
-constexpr float kLimit = 15.0f;    // log2 of the largest weight any reference stays for
-constexpr float kMaxProb = 60.0f;  // log2 of the largest p
+constexpr int kStages = 3;
+// Four CTAs an SM (16 warps) for 16-bit queries of up to 8 rows: the loop is a chain
+// of short latencies, and the warps are what hides them (12 warps: 57% of the issue
+// slots used)
+constexpr float kUp = 10.0f;         // log2 of the largest weight under a new reference
+constexpr float kLimit = 32768.0f;   // largest weight any reference stays for
+constexpr float kMaxProb = 60.0f;    // log2 of the largest p
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async16_if(bool on, uint32_t dst, const void *src) {
+    asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %2, 0;\n @p cp.async.cg.shared.global [%0], [%1], 16;\n}\n" ::"r"(dst),
+                 "l"(src), "r"((uint32_t)on)
+                 : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -132,13 +144,36 @@ __device__ __forceinline__ void lds_words(const uint8_t *p, uint32_t (&w)[N], in
 __device__ __forceinline__ int near_one(float mag) {
     return min(60, max(-60, 127 - (int)((__float_as_uint(mag) >> 23) & 0xffu)));
 }
+// ---- distributed shared memory of a cluster ----
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_addr(uint32_t saddr, uint32_t rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float cluster_ld(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+// The running sum v, l in reference m takes another in reference m1.
+__device__ __forceinline__ void join(float &m, float &l, float (&v)[8], float m1, float l1, const float (&v1)[8]) {
+    const float top = fmaxf(m, m1);
+    const float f = m == top ? 1.0f : pow2_diff(m, top), f1 = m1 == top ? 1.0f : pow2_diff(m1, top);
+    m = top;
+    l = fmaf(l1, f1, l * f);
+#pragma unroll
+    for (int j = 0; j < 8; j++) v[j] = fmaf(v1[j], f1, v[j] * f);
+}
 // Record of row r of a (sequence, KV head) pair and split s: D floats o, then m, l.
 __host__ __device__ inline size_t few_record(uint32_t pair, uint32_t rows, uint32_t r, uint32_t nsplit, uint32_t s) {
     return ((size_t)pair * rows + r) * nsplit + s;
 }
 
 template <int D, int BK, int BV, int NR, bool SPLIT>
-__global__ void __launch_bounds__(kWarps * 32, (NR == 1 && !SPLIT) ? 3 : 2) k_kv_attn_few(KvAttnParams p) {
+__global__ void __launch_bounds__(kWarps * 32, NR == 1 ? (SPLIT ? 3 : 4) : 2) k_kv_attn_few(KvAttnParams p) {
     using T = Tile<D, BK, BV>;
     constexpr int KW = D * BK / 128;       // 32-bit words of a key row per thread
     constexpr int UNITS = D / 32;          // units of eight consecutive elements of a row per thread
@@ -163,7 +198,8 @@ __global__ void __launch_bounds__(kWarps * 32, (NR == 1 && !SPLIT) ? 3 : 2) k_kv
     const KvTiles tiles = kv_tiles(range, kKvFewTile);
     const uint32_t t_begin = split * p.tiles_per_split;
     const uint32_t t_end = min(tiles.total, t_begin + p.tiles_per_split);
-    if (p.nsplit > 1 && t_begin >= t_end) return;  // the merge knows how many parts there are
+    // (whoever joins the parts knows how many there are)
+    if (p.nsplit > 1 && t_begin >= t_end && (split > 0 || !p.cluster)) return;
 
     // ---- copies: lane L of a batch of 32 tiles holds the page of tile L ----
     const uint32_t n_mine = t_begin + warp < t_end ? (t_end - t_begin - warp + kWarps - 1) / kWarps : 0;
@@ -183,36 +219,36 @@ __global__ void __launch_bounds__(kWarps * 32, (NR == 1 && !SPLIT) ? 3 : 2) k_kv
                 page_cur = page_next;
                 page_next = load_page(k + 32 + lane);
             }
-            const uint32_t page = __shfl_sync(0xffffffffu, page_cur, k & 31u);
-            if (page < p.cache.num_pages) {
-                bad &= ~(1u << (k & 31u));
-                const size_t slot = (((size_t)page * p.cache.hkv + h) << p.cache.shift) +
-                                    (tile_token(k) & ((1u << p.cache.shift) - 1u));
-                const uint32_t dst = ring_s + (k % kStages) * T::BYTES;
-                const uint8_t *ks = p.cache.codes[0] + slot * T::RK, *vs = p.cache.codes[1] + slot * T::RV;
-#pragma unroll
-                for (int i = 0; i < (T::K / 16 + 31) / 32; i++) {
-                    const int ch = i * 32 + lane, row = ch / (T::RK / 16), col = ch % (T::RK / 16);
-                    if (T::K / 16 >= 32 || ch < T::K / 16)
-                        cp_async16(dst + row * T::RK + ((col ^ k_swz<T::RK>(row)) * 16), ks + ch * 16);
-                }
-#pragma unroll
-                for (int i = 0; i < (T::V / 16 + 31) / 32; i++) {
-                    const int ch = i * 32 + lane, row = ch / (T::RV / 16), col = ch % (T::RV / 16);
-                    if (T::V / 16 >= 32 || ch < T::V / 16)
-                        cp_async16(dst + T::K + row * T::RV + ((col ^ v_swz<T::RV>(row)) * 16), vs + ch * 16);
-                }
-                if (lane < T::KS / 16)
-                    cp_async16(dst + T::K + T::V + lane * 16,
-                               reinterpret_cast<const uint8_t *>(p.cache.scales[0]) + slot * (T::KS / 16) + lane * 16);
-                if (lane >= 16 && lane < 16 + T::VS / 16)
-                    cp_async16(dst + T::K + T::V + T::KS + (lane - 16) * 16,
-                               reinterpret_cast<const uint8_t *>(p.cache.scales[1]) + slot * (T::VS / 16) +
-                                   (lane - 16) * 16);
-            } else {
+            uint32_t page = __shfl_sync(0xffffffffu, page_cur, k & 31u);
+            bad &= ~(1u << (k & 31u));
+            if (page >= p.cache.num_pages) {
+                // (page 0 is read in its place, and nothing made of it)
                 bad |= 1u << (k & 31u);
                 fault = KV_FAULT_PAGE;
+                page = 0;
             }
+            const size_t slot = (((size_t)page * p.cache.hkv + h) << p.cache.shift) +
+                                (tile_token(k) & ((1u << p.cache.shift) - 1u));
+            const uint32_t dst = ring_s + (k % kStages) * T::BYTES;
+            const uint8_t *ks = p.cache.codes[0] + slot * T::RK + lane * 16, *vs = p.cache.codes[1] + slot * T::RV + lane * 16;
+#pragma unroll
+            for (int i = 0; i < (T::K / 16 + 31) / 32; i++) {
+                const int ch = i * 32 + lane, row = ch / (T::RK / 16), col = ch % (T::RK / 16);
+                cp_async16_if(T::K / 16 >= 32 || ch < T::K / 16, dst + row * T::RK + ((col ^ k_swz<T::RK>(row)) * 16),
+                              ks + i * 512);
+            }
+#pragma unroll
+            for (int i = 0; i < (T::V / 16 + 31) / 32; i++) {
+                const int ch = i * 32 + lane, row = ch / (T::RV / 16), col = ch % (T::RV / 16);
+                cp_async16_if(T::V / 16 >= 32 || ch < T::V / 16, dst + T::K + row * T::RV + ((col ^ v_swz<T::RV>(row)) * 16),
+                              vs + i * 512);
+            }
+            // scales: lanes 0-15 of the keys', 16-31 of the values'
+            const int sl = lane & 15;
+            const uint8_t *ss = lane < 16 ? reinterpret_cast<const uint8_t *>(p.cache.scales[0]) + slot * (T::KS / 16)
+                                          : reinterpret_cast<const uint8_t *>(p.cache.scales[1]) + slot * (T::VS / 16);
+            cp_async16_if(sl < (lane < 16 ? T::KS : T::VS) / 16, dst + T::K + T::V + (lane < 16 ? 0 : T::KS) + sl * 16,
+                          ss + sl * 16);
         }
         cp_commit();
     };
@@ -220,8 +256,14 @@ __global__ void __launch_bounds__(kWarps * 32, (NR == 1 && !SPLIT) ? 3 : 2) k_kv
     for (int k = 0; k < kStages - 1; k++) issue(k);
 
     // ---- queries: row g (+ 8) as the B operand, in the order of the code words ----
+    // 16-bit queries meet the codes as they stand: a code in the low bits of an f16 is
+    // code * 2^-24, exact, and a 4-bit one four bits up 16 times that, which those
+    // elements of the query make up for.  The codes are then not around zero, and the
+    // products cancel against zero - mid * scale, which costs f32 a few units in the
+    // last place of the score (too many for f32 queries, whose codes are centred).
+    constexpr bool RAW = !SPLIT;
     uint32_t qf[NR][NS][KSTEPS][2];
-    float x_scale[NR][2], x_sum[NR][2];  // of this thread's columns, rows 2c and 2c + 1
+    f2 x_scale[NR], x_sum[NR];  // of this thread's columns, rows 2c and 2c + 1
     int x_pos[NR][2];
 #pragma unroll
     for (int nr = 0; nr < NR; nr++) {
@@ -256,12 +298,13 @@ __global__ void __launch_bounds__(kWarps * 32, (NR == 1 && !SPLIT) ? 3 : 2) k_kv
             constexpr int o8[8] = {0, 1, 2, 3, 4, 5, 6, 7}, o4[8] = {0, 4, 1, 5, 2, 6, 3, 7};
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const float v0 = q[u][BK == 8 ? o8[2 * i] : o4[2 * i]] * sc;
-                const float v1 = q[u][BK == 8 ? o8[2 * i + 1] : o4[2 * i + 1]] * sc;
+                const float up = RAW && BK == 4 && (i & 1) ? 16.0f : 1.0f;
+                const float v0 = q[u][BK == 8 ? o8[2 * i] : o4[2 * i]] * (sc / up);
+                const float v1 = q[u][BK == 8 ? o8[2 * i + 1] : o4[2 * i + 1]] * (sc / up);
                 const uint32_t hi = f16x2(v0, v1);
                 const float2 back = f16x2_back(hi);
                 qf[nr][0][2 * u + (i >> 1)][i & 1] = hi;
-                sum += back.x + back.y;
+                sum += (back.x + back.y) * up;
                 if constexpr (SPLIT) {
                     const uint32_t lo = f16x2(v0 - back.x, v1 - back.y);
                     const float2 lb = f16x2_back(lo);
@@ -272,29 +315,39 @@ __global__ void __launch_bounds__(kWarps * 32, (NR == 1 && !SPLIT) ? 3 : 2) k_kv
         }
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        const float xs = p.scale_log2 / sc;
+        // (the sum in the units of the raw products)
+        const float xs = p.scale_log2 / sc * (RAW ? 16777216.0f : 1.0f);
+        if constexpr (RAW) sum *= 1.0f / 16777216.0f;
         const int pos = used ? pos0 + (int)tok : -1;
+        float xe[2], se[2];
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-            x_scale[nr][e] = __shfl_sync(0xffffffffu, xs, (2 * c + e) * 4);
-            x_sum[nr][e] = __shfl_sync(0xffffffffu, sum, (2 * c + e) * 4);
+            xe[e] = __shfl_sync(0xffffffffu, xs, (2 * c + e) * 4);
+            se[e] = __shfl_sync(0xffffffffu, sum, (2 * c + e) * 4);
             x_pos[nr][e] = __shfl_sync(0xffffffffu, pos, (2 * c + e) * 4);
         }
+        x_scale[nr] = pk(xe[0], xe[1]);
+        x_sum[nr] = pk(se[0], se[1]);
     }
 
-    float o[NR][MT][4], m[NR][2], l[NR][2], z[NR][2];
+    float o[NR][MT][4], m[NR][2];
+    f2 l[NR], z[NR], nm[NR];  // nm: minus the reference, 0 while there is none
+    bool unset = false;       // some reference is not set yet
 #pragma unroll
     for (int nr = 0; nr < NR; nr++) {
 #pragma unroll
         for (int j = 0; j < MT; j++)
 #pragma unroll
             for (int i = 0; i < 4; i++) o[nr][j][i] = 0.0f;
+        l[nr] = z[nr] = nm[nr] = pk(0.0f, 0.0f);
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-            m[nr][e] = -INFINITY;
-            l[nr][e] = z[nr][e] = 0.0f;
+            // rows that see nothing start with a reference of their own: they never ask for one
+            m[nr][e] = x_pos[nr][e] >= 0 ? -INFINITY : 0.0f;
+            unset |= m[nr][e] == -INFINITY;
         }
     }
+    unset = __any_sync(0xffffffffu, unset);
 
     // power of two on the values' scales and zeros (0: none of them seen so far but
     // zero) and its reciprocal
@@ -304,8 +357,7 @@ __global__ void __launch_bounds__(kWarps * 32, (NR == 1 && !SPLIT) ? 3 : 2) k_kv
         __syncwarp();
         const uint8_t *st = ring + (k % kStages) * T::BYTES;
         const int j0 = (int)tile_token(k);
-        const bool skip = (bad >> (k & 31u)) & 1u;
-        if (!skip) {
+        if (!((bad >> (k & 31u)) & 1u)) {
             // ---- S^T = K Q^T ----
             uint32_t kw[2][KW];
 #pragma unroll
@@ -326,16 +378,26 @@ __global__ void __launch_bounds__(kWarps * 32, (NR == 1 && !SPLIT) ? 3 : 2) k_kv
             for (int ks = 0; ks < KSTEPS; ks += BK == 8 ? 1 : 2) {
                 if constexpr (BK == 8) {
                     uint32_t a[4];
-                    unpack_u8(kw[0][ks], a[0], a[2]);
-                    unpack_u8(kw[1][ks], a[1], a[3]);
+                    if constexpr (RAW) {
+                        raw_u8(kw[0][ks], a[0], a[2]);
+                        raw_u8(kw[1][ks], a[1], a[3]);
+                    } else {
+                        unpack_u8(kw[0][ks], a[0], a[2]);
+                        unpack_u8(kw[1][ks], a[1], a[3]);
+                    }
 #pragma unroll
                     for (int nr = 0; nr < NR; nr++)
 #pragma unroll
                         for (int n = 0; n < NS; n++) mma16816(s[nr], a, qf[nr][n][ks]);
                 } else {
                     uint32_t u0[4], u1[4];
-                    unpack_u4(kw[0][ks >> 1], u0);
-                    unpack_u4(kw[1][ks >> 1], u1);
+                    if constexpr (RAW) {
+                        raw_u4(kw[0][ks >> 1], u0);
+                        raw_u4(kw[1][ks >> 1], u1);
+                    } else {
+                        unpack_u4(kw[0][ks >> 1], u0);
+                        unpack_u4(kw[1][ks >> 1], u1);
+                    }
 #pragma unroll
                     for (int half = 0; half < 2; half++) {
                         const uint32_t a[4] = {u0[2 * half], u1[2 * half], u0[2 * half + 1], u1[2 * half + 1]};
@@ -347,7 +409,7 @@ __global__ void __launch_bounds__(kWarps * 32, (NR == 1 && !SPLIT) ? 3 : 2) k_kv
                 }
             }
             // ---- scales of tokens j0 + g and j0 + g + 8 ----
-            float sk[2], zk[2], sv[2], zv[2], lv[2];
+            float sk[2], zk[2], sv[2], zv[2];
             const float *kscale = reinterpret_cast<const float *>(st + T::K + T::V);
             const float *vscale = reinterpret_cast<const float *>(st + T::K + T::V + T::KS);
 #pragma unroll
@@ -357,6 +419,7 @@ __global__ void __launch_bounds__(kWarps * 32, (NR == 1 && !SPLIT) ? 3 : 2) k_kv
                 zk[t] = BK == 8 ? 0.0f : kscale[2 * i + 1];
                 sv[t] = BV == 8 ? vscale[i] : vscale[2 * i];
                 zv[t] = BV == 8 ? 0.0f : vscale[2 * i + 1];
+                if constexpr (RAW) zk[t] = fmaf(BK == 8 ? -128.0f : -8.0f, sk[t], zk[t]);
             }
             if (lift == 0.0f) {
                 float mag = 0.0f;
@@ -373,76 +436,120 @@ __global__ void __launch_bounds__(kWarps * 32, (NR == 1 && !SPLIT) ? 3 : 2) k_kv
 #pragma unroll
             for (int t = 0; t < 2; t++) {
                 sv[t] *= lift;
-                zv[t] *= lift;
-                lv[t] = lg2(BV == 8 ? sv[t] : fmaxf(sv[t], fabsf(zv[t])));
+                if constexpr (BV == 4) zv[t] *= lift;
             }
             // every token of the tile seen by every row?
             const bool whole = j0 + (int)kKvFewTile - 1 <= rows.first &&
                                (p.window == 0 || j0 > rows.last - (int)p.window ||
                                 j0 + (int)kKvFewTile <= (int)p.sinks);
-            float x[NR][4];  // [token half t][column e] at 2 t + e
-            bool grow = false;
-#pragma unroll
-            for (int nr = 0; nr < NR; nr++)
-#pragma unroll
-                for (int t = 0; t < 2; t++)
-#pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        float v = s[nr][2 * t + e] * sk[t];
-                        if constexpr (BK == 4) v = fmaf(zk[t], x_sum[nr][e], v);
-                        v *= x_scale[nr][e];
-                        if (!whole && !kv_visible(j0 + g + 8 * t, x_pos[nr][e], (int)p.window, (int)p.sinks))
-                            v = -INFINITY;
-                        x[nr][2 * t + e] = v;
-                        grow |= v > m[nr][e] + kMaxProb || v + lv[t] > m[nr][e] + kLimit;
-                    }
-            if (__any_sync(0xffffffffu, grow)) {
+            // score of token half t and this thread's two rows, before the row's factor
+            auto score = [&](int nr, int t) {
+                const f2 v = mul2(pk(s[nr][2 * t], s[nr][2 * t + 1]), pk(sk[t], sk[t]));
+                return RAW || BK == 4 ? fma2(pk(zk[t], zk[t]), x_sum[nr], v) : v;
+            };
+            uint32_t pf[NR][NS][2];
+            // Weights against the references, first the old ones: true where they hold.
+            auto weigh = [&](auto masked, bool last_try) -> bool {
+                constexpr bool MASK = decltype(masked)::value;
+                f2 pp[NR][2], ww[NR][2];
+                float top = 0.0f;
 #pragma unroll
                 for (int nr = 0; nr < NR; nr++)
 #pragma unroll
+                    for (int t = 0; t < 2; t++) {
+                        float e0, e1;
+                        upk(fma2(score(nr, t), x_scale[nr], nm[nr]), e0, e1);
+                        float v0 = sv[t], v1 = sv[t];
+                        if constexpr (MASK) {
+                            // (a hidden token's values may be anything)
+                            if (!kv_visible(j0 + g + 8 * t, x_pos[nr][0], (int)p.window, (int)p.sinks)) {
+                                e0 = -INFINITY;
+                                v0 = 0.0f;
+                            }
+                            if (!kv_visible(j0 + g + 8 * t, x_pos[nr][1], (int)p.window, (int)p.sinks)) {
+                                e1 = -INFINITY;
+                                v1 = 0.0f;
+                            }
+                        }
+                        const float p0 = ex2(e0), p1 = ex2(e1);
+                        pp[nr][t] = pk(p0, p1);
+                        ww[nr][t] = mul2(pp[nr][t], pk(v0, v1));
+                        float w0, w1;
+                        upk(ww[nr][t], w0, w1);
+                        // a weight above 2^15, or p above 2^60
+                        top = fmaxf(fmaxf(top, fmaxf(w0, w1)), fmaxf(p0, p1) * 2.8421709e-14f);
+                    }
+                if (!last_try && __any_sync(0xffffffffu, top > kLimit)) return false;
+#pragma unroll
+                for (int nr = 0; nr < NR; nr++) {
+                    l[nr] = add2(l[nr], add2(pp[nr][0], pp[nr][1]));
+#pragma unroll
+                    for (int t = 0; t < 2; t++) {
+                        float w0, w1;
+                        upk(ww[nr][t], w0, w1);
+                        if constexpr (BV == 4) {
+                            float p0, p1;
+                            upk(pp[nr][t], p0, p1);
+                            const bool h0 = MASK && p0 == 0.0f, h1 = MASK && p1 == 0.0f;
+                            z[nr] = fma2(pp[nr][t], pk(h0 ? 0.0f : zv[t], h1 ? 0.0f : zv[t]), z[nr]);
+                        }
+                        const uint32_t hi = f16x2(w0, w1);
+                        pf[nr][0][t] = transpose8x8(hi);
+                        if constexpr (SPLIT) {
+                            const float2 back = f16x2_back(hi);
+                            pf[nr][NS - 1][t] = transpose8x8(f16x2(w0 - back.x, w1 - back.y));
+                        }
+                    }
+                }
+                return true;
+            };
+            // References that hold for this tile; the sums so far follow.
+            auto new_reference = [&]() {
+                unset = false;
+#pragma unroll
+                for (int nr = 0; nr < NR; nr++) {
+                    float x[2][2];
+#pragma unroll
+                    for (int t = 0; t < 2; t++) upk(mul2(score(nr, t), x_scale[nr]), x[t][0], x[t][1]);
+                    float cm[2];
+#pragma unroll
                     for (int e = 0; e < 2; e++) {
-                        float mx = fmaxf(x[nr][e], x[nr][2 + e]);
-                        float my = fmaxf(x[nr][e] + lv[0], x[nr][2 + e] + lv[1]);
+                        float mx = -INFINITY, my = -INFINITY;
+#pragma unroll
+                        for (int t = 0; t < 2; t++)
+                            if (whole || kv_visible(j0 + g + 8 * t, x_pos[nr][e], (int)p.window, (int)p.sinks)) {
+                                mx = fmaxf(mx, x[t][e]);
+                                my = fmaxf(my, x[t][e] + lg2(BV == 8 ? sv[t] : fmaxf(sv[t], fabsf(zv[t]))));
+                            }
 #pragma unroll
                         for (int w = 4; w < 32; w <<= 1) {
                             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
                             my = fmaxf(my, __shfl_xor_sync(0xffffffffu, my, w));
                         }
-                        // (a reference is only moved up, and only where this tile needs it)
-                        float m1 = fmaxf(m[nr][e], ceilf(mx) - kMaxProb);
-                        if (my > m1 + kLimit || m1 == -INFINITY) m1 = fmaxf(m1, ceilf(my) - kUp);
-                        const float cm = m1 == m[nr][e] ? 1.0f : pow2_diff(m[nr][e], m1);
-                        l[nr][e] *= cm;
-                        z[nr][e] *= cm;
+                        const float m1 = fmaxf(m[nr][e], fmaxf(ceilf(mx) - kMaxProb, ceilf(my) - kUp));
+                        cm[e] = m1 == m[nr][e] ? 1.0f : pow2_diff(m[nr][e], m1);
                         m[nr][e] = m1;
-#pragma unroll
-                        for (int j = 0; j < MT; j++) {
-                            o[nr][j][e] *= cm;
-                            o[nr][j][2 + e] *= cm;
-                        }
+                        unset |= m1 == -INFINITY;
                     }
-            }
-            uint32_t pf[NR][NS][2];
+                    nm[nr] = pk(m[nr][0] == -INFINITY ? 0.0f : -m[nr][0], m[nr][1] == -INFINITY ? 0.0f : -m[nr][1]);
+                    l[nr] = mul2(l[nr], pk(cm[0], cm[1]));
+                    z[nr] = mul2(z[nr], pk(cm[0], cm[1]));
 #pragma unroll
-            for (int nr = 0; nr < NR; nr++)
+                    for (int j = 0; j < MT; j++)
 #pragma unroll
-                for (int t = 0; t < 2; t++) {
-                    float w[2];
-#pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        const float v = x[nr][2 * t + e];
-                        const float pr = v == -INFINITY ? 0.0f : ex2(v - m[nr][e]);
-                        l[nr][e] += pr;
-                        if (BV == 4 && pr != 0.0f) z[nr][e] = fmaf(pr, zv[t], z[nr][e]);
-                        w[e] = pr == 0.0f ? 0.0f : pr * sv[t];
-                    }
-                    const uint32_t hi = f16x2(w[0], w[1]);
-                    pf[nr][0][t] = transpose8x8(hi);
-                    if constexpr (SPLIT) {
-                        const float2 back = f16x2_back(hi);
-                        pf[nr][NS - 1][t] = transpose8x8(f16x2(w[0] - back.x, w[1] - back.y));
-                    }
+                        for (int i = 0; i < 4; i++) o[nr][j][i] *= cm[i & 1];
                 }
+                unset = __any_sync(0xffffffffu, unset);
+            };
+            bool renew = unset, last_try = false;
+            while (true) {
+                if (renew) {
+                    new_reference();
+                    last_try = true;
+                }
+                if (whole ? weigh(std::false_type{}, last_try) : weigh(std::true_type{}, last_try)) break;
+                renew = true;
+            }
             // ---- O^T += V^T P^T: tokens 2c, 2c + 1, 2c + 8, 2c + 9, dims g * D/8 .. ----
             constexpr int VW = T::RV / 32;  // words per token (0: two bytes)
             const uint8_t *vr = st + T::K;
@@ -521,6 +628,7 @@ __global__ void __launch_bounds__(kWarps * 32, (NR == 1 && !SPLIT) ? 3 : 2) k_kv
     cp_wait<0>();
     if (fault && lane == 0) kv_report(p.fault, fault);
 
+    pdl_launch_dependents();
     // ---- join the warps: records of (row, dim) in the first one's reference ----
     __syncthreads();
     constexpr int RS = D + 2;
@@ -529,7 +637,9 @@ __global__ void __launch_bounds__(kWarps * 32, (NR == 1 && !SPLIT) ? 3 : 2) k_kv
     for (int nr = 0; nr < NR; nr++)
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-            float lt = l[nr][e], zt = z[nr][e];
+            float lt, zt, other;
+            upk(l[nr], e ? other : lt, e ? lt : other);
+            upk(z[nr], e ? other : zt, e ? zt : other);
 #pragma unroll
             for (int w = 4; w < 32; w <<= 1) {
                 lt += __shfl_xor_sync(0xffffffffu, lt, w);
@@ -548,51 +658,74 @@ __global__ void __launch_bounds__(kWarps * 32, (NR == 1 && !SPLIT) ? 3 : 2) k_kv
         }
     __syncthreads();
     const uint32_t pair = (b * p.cache.hkv + h) * p.row_tiles + rt;
+    float *mine = rec + kWarps * 8 * NR * RS;  // this part's records, for the cluster
+    auto finish = [&](uint32_t r, uint32_t d0, float l_all, float(&v)[8]) {
+        const float inv = l_all == 0.0f ? 0.0f : 1.0f / l_all;
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] *= inv;
+        const uint32_t tok = (rows.r0 + r) / G, head = h * G + (rows.r0 + r) % G;
+        store8(p.out.data, (size_t)(seq.q0 + tok) * p.out.row_stride + head * p.out.head_stride + d0, p.out.fmt, v);
+    };
     for (uint32_t i = threadIdx.x; i < rows.n * (D / 8); i += kWarps * 32) {
         const uint32_t r = i / (D / 8), d0 = (i % (D / 8)) * 8;
-        float top = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < kWarps; w++) top = fmaxf(top, rec[(w * 8 * NR + r) * RS + D]);
-        float v[8] = {0, 0, 0, 0, 0, 0, 0, 0}, lsum = 0.0f;
+        float top = -INFINITY, l_all = 0.0f, v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
         for (int w = 0; w < kWarps; w++) {
             const float *src = rec + (w * 8 * NR + r) * RS;
-            if (src[D] == -INFINITY && !(src[D + 1] != src[D + 1])) continue;
-            const float f = src[D] == top ? 1.0f : pow2_diff(src[D], top);
-            lsum = fmaf(src[D + 1], f, lsum);
+            float v1[8];
 #pragma unroll
-            for (int j = 0; j < 8; j++) v[j] = fmaf(src[d0 + j], f, v[j]);
+            for (int j = 0; j < 8; j++) v1[j] = src[d0 + j];
+            join(top, l_all, v, src[D], src[D + 1], v1);
         }
         if (p.nsplit > 1) {
-            float *dst = p.part + few_record(pair, R, r, p.nsplit, split) * RS;
+            float *dst = p.cluster ? mine + r * RS : p.part + few_record(pair, R, r, p.nsplit, split) * RS;
 #pragma unroll
-            for (int j = 0; j < 8; j++) dst[d0 + j] = v[j];
-            if (d0 == 0) {
-                dst[D] = top;
-                dst[D + 1] = lsum;
-            }
+            for (int j = 0; j < 8; j += 2) *reinterpret_cast<float2 *>(dst + d0 + j) = make_float2(v[j], v[j + 1]);
+            if (d0 == 0) *reinterpret_cast<float2 *>(dst + D) = make_float2(top, l_all);
         } else {
-            const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;
-#pragma unroll
-            for (int j = 0; j < 8; j++) v[j] *= inv;
-            const uint32_t tok = (rows.r0 + r) / G, head = h * G + (rows.r0 + r) % G;
-            store8(p.out.data, (size_t)(seq.q0 + tok) * p.out.row_stride + head * p.out.head_stride + d0, p.out.fmt, v);
+            finish(r, d0, l_all, v);
         }
+    }
+    if (p.cluster && p.nsplit > 1) {
+        const uint32_t used = max(1u, (tiles.total + p.tiles_per_split - 1) / p.tiles_per_split);
+        cluster_sync();
+        for (uint32_t i = split * (kWarps * 32) + threadIdx.x; i < rows.n * (D / 8); i += used * (kWarps * 32)) {
+            const uint32_t r = i / (D / 8), d0 = (i % (D / 8)) * 8;
+            float top = -INFINITY, l_all = 0.0f, v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+            for (uint32_t s = 0; s < used; s++) {
+                const uint32_t src = cluster_addr(smem_u32(mine + r * RS), s);
+                float v1[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) v1[j] = cluster_ld(src + 4 * (d0 + j));
+                join(top, l_all, v, cluster_ld(src + 4 * D), cluster_ld(src + 4 * D + 4), v1);
+            }
+            finish(r, d0, l_all, v);
+        }
+        cluster_sync();  // nobody leaves while its records are read
     }
 }
 
 template <int D, int BK, int BV, int NR, bool SPLIT>
 cudaError_t launch_few_t(const KvAttnParams &p, cudaStream_t st) {
     using T = Tile<D, BK, BV>;
-    constexpr int JOIN = kWarps * 8 * NR * (D + 2) * 4;
+    constexpr int JOIN = (kWarps + 1) * 8 * NR * (D + 2) * 4;
     constexpr int SMEM = T::SMEM > JOIN ? T::SMEM : JOIN;
     auto *fn = k_kv_attn_few<D, BK, BV, NR, SPLIT>;
     if (SMEM > 48 * 1024) {
         cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
         if (e != cudaSuccess) return e;
     }
-    fn<<<dim3(p.nsplit * p.row_tiles, p.cache.hkv, p.batch.n_seqs), kWarps * 32, SMEM, st>>>(p);
-    return cudaGetLastError();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(p.nsplit * p.row_tiles, p.cache.hkv, p.batch.n_seqs);
+    cfg.blockDim = dim3(kWarps * 32);
+    cfg.dynamicSmemBytes = SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim = {p.nsplit, 1, 1};
+    cfg.attrs = attr;
+    cfg.numAttrs = p.cluster && p.nsplit > 1 ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, fn, p);
 }
 
 template <int D, int BK, int BV>

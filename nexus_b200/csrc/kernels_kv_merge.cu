@@ -6,9 +6,9 @@
 // powers of two).  A block joins one row: D / 8 lanes own eight dims each and
 // the groups of lanes take the splits in turn, each a running sum in the
 // largest reference so far; the groups' sums are then added in order.  The
-// order depends on the number of splits alone.  Bound by latency: two rounds
-// of loads a group where a single lane would wait for every split in turn
-// (222 splits of one row took most of 229 us so).
+// order depends on the number of splits alone.  Bound by latency: four records
+// of a group are loaded at once (one lane waiting for every split in turn took
+// most of 229 us for 222 splits of a row).
 #include "kernels_kv_few.cuh"
 
 namespace nx {
@@ -39,21 +39,13 @@ cudaError_t launch_kv_attn_chunk(const KvAttnParams &p, cudaStream_t st) {
 }
 
 constexpr int kMergeThreads = 128;
-
-// The running sum v, l in reference m takes another in reference m1.
-__device__ __forceinline__ void join(float &m, float &l, float (&v)[8], float m1, float l1, const float (&v1)[8]) {
-    const float top = fmaxf(m, m1);
-    const float f = m == top ? 1.0f : kvf::pow2_diff(m, top), f1 = m1 == top ? 1.0f : kvf::pow2_diff(m1, top);
-    m = top;
-    l = fmaf(l1, f1, l * f);
-#pragma unroll
-    for (int j = 0; j < 8; j++) v[j] = fmaf(v1[j], f1, v[j] * f);
-}
+using kvf::join;
 
 template <int D>
 __global__ void __launch_bounds__(kMergeThreads) k_kv_merge(KvAttnParams p) {
     constexpr int RS = D + 2, LANES = D / 8, GROUPS = kMergeThreads / LANES;
     __shared__ float sm_m[GROUPS], sm_l[GROUPS], sm_v[GROUPS][D];
+    pdl_wait();  // (launched while the parts' last CTAs run)
     const uint32_t b = blockIdx.y, h = blockIdx.x / p.row_tiles, rt = blockIdx.x % p.row_tiles, r = blockIdx.z;
     unsigned fault = 0;
     const KvSeqView seq = kv_load_seq(p.batch, b, p.cache.shift, &fault);  // reported by the parts
@@ -68,17 +60,26 @@ __global__ void __launch_bounds__(kMergeThreads) k_kv_merge(KvAttnParams p) {
     const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES, d0 = 8 * lane;
     const float *src = p.part + kvf::few_record(tile, p.tile_rows, r, p.nsplit, 0) * RS;
     float m = -INFINITY, l = 0.0f, v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    for (uint32_t s = group; s < used; s += GROUPS) {
-        const float *part = src + (size_t)s * RS;
-        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(part + D));
-        float v1[8];
+    // four records of a group in flight at once
+#pragma unroll 1
+    for (uint32_t s0 = group; s0 < used; s0 += 4 * GROUPS) {
+        float2 ml[4];
+        float v1[4][8];
 #pragma unroll
-        for (int j = 0; j < 8; j += 2) {
-            const float2 t = __ldcg(reinterpret_cast<const float2 *>(part + d0 + j));
-            v1[j] = t.x;
-            v1[j + 1] = t.y;
+        for (int u = 0; u < 4; u++) {
+            if (s0 + u * GROUPS >= used) continue;
+            const float *part = src + (size_t)(s0 + u * GROUPS) * RS;
+            ml[u] = __ldcg(reinterpret_cast<const float2 *>(part + D));
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) {
+                const float2 t = __ldcg(reinterpret_cast<const float2 *>(part + d0 + j));
+                v1[u][j] = t.x;
+                v1[u][j + 1] = t.y;
+            }
         }
-        join(m, l, v, ml.x, ml.y, v1);
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+            if (s0 + u * GROUPS < used) join(m, l, v, ml[u].x, ml[u].y, v1[u]);
     }
     if (lane == 0) {
         sm_m[group] = m;
@@ -103,14 +104,21 @@ __global__ void __launch_bounds__(kMergeThreads) k_kv_merge(KvAttnParams p) {
 }
 
 cudaError_t launch_kv_merge(const KvAttnParams &p, cudaStream_t st) {
-    const dim3 grid(p.cache.hkv * p.row_tiles, p.batch.n_seqs, p.tile_rows);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(p.cache.hkv * p.row_tiles, p.batch.n_seqs, p.tile_rows);
+    cfg.blockDim = dim3(kMergeThreads);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
     switch (p.cache.head_dim) {
-    case 32: k_kv_merge<32><<<grid, kMergeThreads, 0, st>>>(p); break;
-    case 64: k_kv_merge<64><<<grid, kMergeThreads, 0, st>>>(p); break;
-    case 128: k_kv_merge<128><<<grid, kMergeThreads, 0, st>>>(p); break;
+    case 32: return cudaLaunchKernelEx(&cfg, k_kv_merge<32>, p);
+    case 64: return cudaLaunchKernelEx(&cfg, k_kv_merge<64>, p);
+    case 128: return cudaLaunchKernelEx(&cfg, k_kv_merge<128>, p);
     default: return cudaErrorInvalidValue;
     }
-    return cudaGetLastError();
 }
 
 }  // namespace nx

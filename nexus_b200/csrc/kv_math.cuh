@@ -93,11 +93,72 @@ __device__ __forceinline__ void unpack_u4(uint32_t w, uint32_t (&p)[4]) {
     p[3] = kv_hfma2(kv_field(s, 0x00f000f0u), 0x2c002c00u, 0xd480d480u);
 }
 
+// The same codes as they stand, in the low bits of f16 (code * 2^-24): pairs (0, 1),
+// (2, 3) of a word of 8-bit codes; (0, 4), 16 * (1, 5), (2, 6), 16 * (3, 7) of 4-bit ones
+__device__ __forceinline__ void raw_u8(uint32_t w, uint32_t &p01, uint32_t &p23) {
+    asm("prmt.b32 %0, %1, 0, 0x4140;" : "=r"(p01) : "r"(w));
+    asm("prmt.b32 %0, %1, 0, 0x4342;" : "=r"(p23) : "r"(w));
+}
+__device__ __forceinline__ void raw_u4(uint32_t w, uint32_t (&p)[4]) {
+    const uint32_t s = w >> 8;
+    p[0] = w & 0x000f000fu;
+    p[1] = w & 0x00f000f0u;
+    p[2] = s & 0x000f000fu;
+    p[3] = s & 0x00f000f0u;
+}
+
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+
+// ---- packed pairs of f32 (two results an instruction) ----
+typedef unsigned long long f2;
+__device__ __forceinline__ f2 pk(float a, float b) {
+    f2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void upk(f2 v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+    f2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f2 add2(f2 a, f2 b) {
+    f2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+    f2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
+__device__ __forceinline__ float4 lds4(uint32_t a) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ f2 lds2(uint32_t a) {
+    f2 v;
+    asm volatile("ld.shared.b64 %0, [%1];" : "=l"(v) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ float lds1(uint32_t a) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ void sts1(uint32_t a, float v) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory"); }
+__device__ __forceinline__ void sts4(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+__device__ __forceinline__ float max4(float4 v) { return fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)); }
+// the first n of 32 bits, any n
+__device__ __forceinline__ uint32_t first_bits(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
 
 // The power of two that brings a row whose largest magnitude is `amax` to
 // [2^7, 2^8): the queries then fit f16 with 22 significant bits in hi + lo,
