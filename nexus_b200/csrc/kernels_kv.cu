@@ -74,7 +74,7 @@ __device__ __forceinline__ void kv_check_batch(const KvCopyParams &p) {
 // subtracting 1.5 * 2^23, whose low byte is the code, and what is rare is looked
 // for once a thread: a quotient near a tie, a value that is not a number.
 template <int D, int BITS>
-__device__ __forceinline__ void kv_quantise_group(const float (&x)[8], uint8_t *codes, float *scales, int64_t slot, int sub,
+__device__ __forceinline__ void kv_quantise_group(float (&x)[8], uint8_t *codes, float *scales, int64_t slot, int sub,
                                                   unsigned lanes) {
     constexpr int LANES = D / 8;
     constexpr float kRound = 12582912.0f;
@@ -110,24 +110,27 @@ __device__ __forceinline__ void kv_quantise_group(const float (&x)[8], uint8_t *
         for (int i = 0; i < 8; i++) t[i] = __float_as_uint(kRound);
         if (!finite) scale = zero = kv_nan();
     } else {
-        const bool tiny = scale < 1e-30f;  // the reciprocal would leave f32
-        const float inv = tiny ? 0.0f : __fdividef(1.0f, scale);
+        float step = scale, mid = zero;
+        if (scale < 1e-30f) {
+            // so that the reciprocal stays in f32: by 2^96, exactly (elements that span so
+            // little are as small themselves)
+            constexpr float kUp96 = 7.9228163e28f;
+            step *= kUp96;
+            mid *= kUp96;
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] *= kUp96;
+        }
+        const float inv = __fdividef(1.0f, step);
         float far = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            float q = (BITS == 8 ? x[i] : __fsub_rn(x[i], zero)) * inv;
+            float q = (BITS == 8 ? x[i] : __fsub_rn(x[i], mid)) * inv;
             if constexpr (BITS == 4) q = fminf(fmaxf(q, low), high);  // (a rounded zero can shift the range)
             const float r = __fadd_rn(q, kRound);
             far = fmaxf(far, fabsf(q - __fsub_rn(r, kRound)));
             t[i] = __float_as_uint(r);
         }
-        if (tiny) {
-#pragma unroll 1
-            for (int i = 0; i < 8; i++) {
-                const double q = rint(((double)x[i] - (double)zero) / (double)scale);
-                t[i] = __float_as_uint(kRound + (float)fmin(fmax(q, (double)low), (double)high));
-            }
-        } else if (far > 0.4999f) {
+        if (far > 0.4999f) {
             // Near a tie (common: coarse inputs meet ties exactly) the remainder decides, in
             // f32 without an error: d + e = x - zero by two-sum, d - code * scale is a
             // multiple of scale's last place below scale, and its difference to scale / 2
@@ -137,12 +140,12 @@ __device__ __forceinline__ void kv_quantise_group(const float (&x)[8], uint8_t *
                 const float code = __fsub_rn(__uint_as_float(t[i]), kRound);
                 float d = x[i], e = 0.0f;
                 if constexpr (BITS == 4) {
-                    d = __fsub_rn(x[i], zero);
+                    d = __fsub_rn(x[i], mid);
                     const float bb = __fsub_rn(d, x[i]);
-                    e = __fadd_rn(__fsub_rn(x[i], __fsub_rn(d, bb)), -__fadd_rn(zero, bb));
+                    e = __fadd_rn(__fsub_rn(x[i], __fsub_rn(d, bb)), -__fadd_rn(mid, bb));
                 }
-                const float left = __fmaf_rn(-code, scale, d), side = left < 0.0f ? -1.0f : 1.0f;
-                const float over = __fadd_rn(__fsub_rn(fabsf(left), 0.5f * scale), side * e);
+                const float left = __fmaf_rn(-code, step, d), side = left < 0.0f ? -1.0f : 1.0f;
+                const float over = __fadd_rn(__fsub_rn(fabsf(left), 0.5f * step), side * e);
                 const bool odd_code = t[i] & 1u;
                 float c = code;
                 if (over > 0.0f || (over == 0.0f && odd_code)) c = __fadd_rn(code, side);
@@ -166,7 +169,7 @@ __device__ __forceinline__ void kv_quantise_group(const float (&x)[8], uint8_t *
 }
 
 template <int D>
-__global__ void __launch_bounds__(kKvCopyThreads) k_kv_append(KvCopyParams p) {
+__global__ void __launch_bounds__(kKvCopyThreads, 5) k_kv_append(KvCopyParams p) {
     constexpr int LANES = D / 8;
     KvPlace<D> at(p);
     // the elements are on their way while the slot is looked up
@@ -207,12 +210,13 @@ __global__ void __launch_bounds__(kKvCopyThreads) k_kv_read(KvCopyParams p) {
             const float scale = p.cache.scales[s][slot];
 #pragma unroll
             for (int i = 0; i < 8; i++)
-                v[i] = __fmul_rn((float)((int)(((i < 4 ? w.x : w.y) >> (8 * (i & 3))) & 0xffu) - 128), scale);
+                // 2^23 + code as f32 bits, less 2^23 + 128
+                v[i] = __fmul_rn(__fsub_rn(__uint_as_float(__byte_perm(i < 4 ? w.x : w.y, 0x4b000000u, 0x7540 | (i & 3))), 8388736.0f), scale);
         } else {
             const uint32_t w = *reinterpret_cast<const uint32_t *>(p.cache.codes[s] + (size_t)slot * (D / 2) + sub * 4);
             const float2 sz = *reinterpret_cast<const float2 *>(p.cache.scales[s] + 2 * slot);
 #pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = __fmaf_rn(sz.x, (float)((int)((w >> (4 * i)) & 0xfu) - 8), sz.y);
+            for (int i = 0; i < 8; i++) v[i] = __fmaf_rn(sz.x, __fsub_rn(__uint_as_float(((w >> (4 * i)) & 0xfu) | 0x4b000000u), 8388616.0f), sz.y);
         }
         store8(p.rows[s].data, at.element(p.rows[s]), p.rows[s].fmt, v);
     }

@@ -28,6 +28,7 @@ from . import _lib as L
 from .engine import CudaBackend
 
 _FORMATS = {torch.float32: L.F32, torch.float16: L.F16, torch.bfloat16: L.BF16}
+_raw_stream = torch._C._cuda_getCurrentRawStream  # torch.cuda.current_stream().cuda_stream without its object
 
 
 def _invalid(msg: str) -> L.NexusError:
@@ -70,9 +71,15 @@ class KvBatch:
         self.max_q, self.max_kv = int(max_q), int(max_kv)
         self._args = (n, self.max_q, self.max_kv, page_table.stride(0) if n > 1 else page_table.shape[1],
                       q_start.data_ptr(), kv_len.data_ptr(), page_table.data_ptr())
+        self._index = kv_len.get_device()
+        self._structs = {}     # by stream: filled once, never changed
+        self._workspaces = {}  # bytes by what they depend on
 
-    def _struct(self, stream: int) -> L.KvBatch:
-        return L.KvBatch(*self._args, stream, L.KV_CALLER_STREAM)
+    def _ref(self, stream: int):
+        r = self._structs.get(stream)
+        if r is None:
+            r = self._structs[stream] = C.byref(L.KvBatch(*self._args, stream, L.KV_CALLER_STREAM))
+        return r
 
 
 class PagedKvCache:
@@ -105,6 +112,7 @@ class PagedKvCache:
         self._struct = L.KvCache(self.kv_heads, self.head_dim, self.page_tokens, self.num_pages, bits[0], bits[1],
                                  k_codes.data_ptr(), v_codes.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr())
         self._ref = C.byref(self._struct)
+        self._shape = (self.kv_heads, self.head_dim, self.page_tokens, self.bits)
         self._lib = backend._lib
 
     @classmethod
@@ -121,35 +129,33 @@ class PagedKvCache:
             buffers.append(torch.zeros((*shape, 1 if b == 8 else 2), dtype=torch.float32, device=dev))
         return cls(backend, *buffers)
 
-    def _stream(self) -> int:
-        return torch.cuda.current_stream(self.device).cuda_stream
-
-    def _batch(self, batch: KvBatch, stream: int) -> L.KvBatch:
-        if batch.kv_len.device != self.device:
-            raise _invalid(f"the batch is on {batch.kv_len.device}, the backend on {self.device}")
-        return batch._struct(stream)
+    def _batch(self, batch: KvBatch):
+        if batch._index != self.backend.device:
+            raise _invalid(f"the batch is on cuda:{batch._index}, the backend on {self.device}")
+        return batch._ref(_raw_stream(self.backend.device))
 
     def _rows(self, t: torch.Tensor, what: str) -> L.KvRows:
         fmt = _FORMATS.get(t.dtype)
         if fmt is None:
             raise _invalid(f"{what} must be float32, float16 or bfloat16")
-        if t.dim() != 3 or t.shape[2] != self.head_dim:
+        shape = t.shape
+        if len(shape) != 3 or shape[2] != self.head_dim:
             raise _invalid(f"{what} must be [rows, heads, {self.head_dim}]")
-        if t.numel() and t.stride(2) != 1:
+        n, h, d = shape
+        rs, hs, es = t.stride()
+        if es != 1 and n and h:
             raise _invalid(f"{what}: the elements of a head must be adjacent")
-        if t.device != self.device:
+        if not t.is_cuda or t.get_device() != self.backend.device:
             raise _invalid(f"{what} is on {t.device}, the backend on {self.device}")
         # a dimension of one has no stride that matters
-        rs = t.stride(0) if t.shape[0] > 1 else self.head_dim * t.shape[1]
-        hs = t.stride(1) if t.shape[1] > 1 else self.head_dim
-        return L.KvRows(t.data_ptr(), fmt, t.shape[1], t.shape[0], rs, hs)
+        return L.KvRows(t.data_ptr(), fmt, h, n, rs if n > 1 else d * h, hs if h > 1 else d)
 
     def append(self, batch: KvBatch, k: torch.Tensor, v: torch.Tensor) -> None:
         """Quantise the batch's rows of k and v ([rows, kv_heads, head_dim]) into their slots."""
-        bt = self._batch(batch, self._stream())
-        rk, rv = self._rows(k, "k"), self._rows(v, "v")
-        L.check(self._lib.nexus_cuda_kv_append(self.backend.handle, self._ref, C.byref(bt), C.byref(rk), C.byref(rv)),
-                self.backend.handle)
+        bt, rk, rv = self._batch(batch), self._rows(k, "k"), self._rows(v, "v")
+        rc = self._lib.nexus_cuda_kv_append(self.backend.handle, self._ref, bt, C.byref(rk), C.byref(rv))
+        if rc:
+            L.check(rc, self.backend.handle)
 
     def read(self, batch: KvBatch, rows: int, dtype: torch.dtype = torch.float32,
              out: Optional[tuple[torch.Tensor, torch.Tensor]] = None) -> tuple[torch.Tensor, torch.Tensor]:
@@ -157,14 +163,16 @@ class PagedKvCache:
         [rows, kv_heads, head_dim].  Rows outside every sequence are left as
         they were (undefined without `out`)."""
         if out is None:
-            out = tuple(torch.empty((rows, self.kv_heads, self.head_dim), dtype=dtype, device=self.device)
-                        for _ in range(2))
-        bt = self._batch(batch, self._stream())
+            shape = (rows, self.kv_heads, self.head_dim)
+            out = (torch.empty(shape, dtype=dtype, device=self.device),
+                   torch.empty(shape, dtype=dtype, device=self.device))
+        bt = self._batch(batch)
         rk, rv = self._rows(out[0], "k"), self._rows(out[1], "v")
         if rk.rows != rows or rv.rows != rows:
             raise _invalid(f"out must have {rows} rows")
-        L.check(self._lib.nexus_cuda_kv_read(self.backend.handle, self._ref, C.byref(bt), C.byref(rk), C.byref(rv)),
-                self.backend.handle)
+        rc = self._lib.nexus_cuda_kv_read(self.backend.handle, self._ref, bt, C.byref(rk), C.byref(rv))
+        if rc:
+            L.check(rc, self.backend.handle)
         return out
 
     def attention(self, batch: KvBatch, q: torch.Tensor, scale: Optional[float] = None, window: int = 0,
@@ -177,20 +185,25 @@ class PagedKvCache:
             raise _invalid("window and sinks must not be negative")
         if out is None:
             out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
-        bt = self._batch(batch, self._stream())
-        rq, ro = self._rows(q, "q"), self._rows(out, "out")
-        need = C.c_size_t()
-        L.check(self._lib.nexus_cuda_kv_attention_workspace(self._ref, C.byref(bt), C.byref(rq), window, sinks,
-                                                            C.byref(need)))
-        ws = torch.empty(need.value, dtype=torch.uint8, device=self.device) if need.value else None
-        L.check(self._lib.nexus_cuda_kv_attention(self.backend.handle, self._ref, C.byref(bt), C.byref(rq),
-                                                  C.byref(ro), 0.0 if scale is None else scale, window, sinks,
-                                                  None if ws is None else ws.data_ptr(), need.value),
-                self.backend.handle)
+        bt, rq, ro = self._batch(batch), self._rows(q, "q"), self._rows(out, "out")
+        qr = C.byref(rq)
+        key = (rq.heads, rq.format, rq.rows > 0, window, sinks, self._shape)
+        need = batch._workspaces.get(key)
+        if need is None:
+            size = C.c_size_t()
+            L.check(self._lib.nexus_cuda_kv_attention_workspace(self._ref, bt, qr, window, sinks, C.byref(size)))
+            need = batch._workspaces[key] = size.value
+        # (held until the launch; reused by the allocator in stream order after it)
+        ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+        rc = self._lib.nexus_cuda_kv_attention(self.backend.handle, self._ref, bt, qr, C.byref(ro),
+                                               0.0 if scale is None else scale, window, sinks,
+                                               None if ws is None else ws.data_ptr(), need)
+        if rc:
+            L.check(rc, self.backend.handle)
         return out
 
     def status(self) -> None:
         """Wait for torch's current stream; raise NexusError for what the calls
         of this backend found wrong on the device (then cleared)."""
-        L.check(self._lib.nexus_cuda_kv_status(self.backend.handle, self._stream(), L.KV_CALLER_STREAM),
+        L.check(self._lib.nexus_cuda_kv_status(self.backend.handle, _raw_stream(self.backend.device), L.KV_CALLER_STREAM),
                 self.backend.handle)
