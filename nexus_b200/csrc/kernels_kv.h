@@ -45,7 +45,7 @@ struct KvAttnParams {
     unsigned *fault;
     // split over the context
     uint32_t nsplit, tiles_per_split;
-    float *part;               // records of unfinished softmaxes (nsplit > 1)
+    float *part, *ml;          // records of unfinished softmaxes (nsplit > 1): D sums; reference, sum of p
     float *sums;               // chunk kernel, f32 queries: a CTA's output sums
     // sequences of at most rows_limit (token, head) rows per KV head are the
     // few-row kernel's, the others the chunk kernel's

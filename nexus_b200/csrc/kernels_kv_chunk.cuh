@@ -693,70 +693,70 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
             const float l = row_x[in_tile], z = row_sum[in_tile];
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             const uint32_t tile_id = (b * p.cache.hkv + h) * p.row_tiles + rt;
-            float *rec = p.nsplit > 1 ? p.part + kvf::few_record(tile_id, kRows, in_tile, p.nsplit, split) * (D + 2)
-                                      : nullptr;
-            // Finished rows go through the warp's quarter of its Q tile (every product has
-            // completed), 16-byte chunks XORed with the row, so that a row leaves in whole
-            // lines; parts of a split go out as they are.
-            constexpr int ES = SPLIT ? 4 : 2, ROWB = D * ES, CPR = ROWB / 16;  // bytes, chunks of a row
-            constexpr int SWZ = CPR < 8 ? CPR - 1 : 7;
-            const uint32_t stage = sbase + sub * S::Q_SUB + wq * (S::Q_SUB / 4);
-            static_assert(32 * ROWB <= S::Q_SUB / 4, "a warp's rows fit its quarter of Q");
+            const bool split_part = p.nsplit > 1;
+            // Rows go through the warp's quarter of its Q tile (every product has completed),
+            // 16-byte chunks XORed with the row, so that a row leaves in whole lines: in the
+            // output's type, or the f32 sums of a part, half of the dims at a time where
+            // the quarter holds no more.
+            constexpr int ES = SPLIT ? 4 : 2, STAGE = S::Q_SUB / 4, DP = 32 * D * 4 > STAGE ? D / 2 : D;
+            static_assert(32 * D * ES <= STAGE && 32 * DP * 4 <= STAGE, "a warp's rows fit its quarter of Q");
+            const uint32_t stage = sbase + sub * S::Q_SUB + wq * STAGE;
+            const uint32_t rec0 = ((b * p.cache.hkv + h) * p.row_tiles + rt) * kRows;
+            auto record = [&](uint32_t row) { return ((size_t)rec0 + row) * p.nsplit + split; };
+            const int wide = split_part ? 4 : ES, pass_dims = split_part ? DP : D;
+            const int cpr = pass_dims * wide / 16, swz = min(cpr, 8) - 1;  // chunks of a staged row
 #pragma unroll 1
-            for (int d0 = 0; d0 < D; d0 += 32) {
-                float o[32];
-                if (cnt > 0) {
-                    tmem_ld_rows32(ocol + d0, o);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 32; j++) o[j] = 0.0f;
-                }
-#pragma unroll
-                for (int u = 0; u < 4; u++) {
-                    // positions of elements 0..7 within a unit of value codes
-                    constexpr int i8[8] = {0, 1, 2, 3, 4, 5, 6, 7}, i4[8] = {0, 2, 4, 6, 1, 3, 5, 7};
-                    float v[8];
-#pragma unroll
-                    for (int e = 0; e < 8; e++) v[e] = (o[8 * u + (BV == 8 ? i8[e] : i4[e])] + z) * unit;
-                    if (rec) {
-                        if (valid) {
-#pragma unroll
-                            for (int e = 0; e < 8; e += 2)
-                                *reinterpret_cast<float2 *>(rec + d0 + 8 * u + e) = make_float2(v[e], v[e + 1]);
-                        }
+            for (int p0 = 0; p0 < D; p0 += pass_dims) {
+                __syncwarp();
+#pragma unroll 1
+                for (int d0 = p0; d0 < p0 + pass_dims; d0 += 32) {
+                    float o[32];
+                    if (cnt > 0) {
+                        tmem_ld_rows32(ocol + d0, o);
                     } else {
 #pragma unroll
-                        for (int e = 0; e < 8; e++) v[e] *= inv;
-                        const uint32_t row = stage + lane * ROWB;
-                        const int ch = (d0 + 8 * u) * ES / 16;
-                        if constexpr (SPLIT) {
-                            sts4(row + ((ch ^ (lane & SWZ)) << 4), __float_as_uint(v[0]), __float_as_uint(v[1]),
+                        for (int j = 0; j < 32; j++) o[j] = 0.0f;
+                    }
+                    const uint32_t row = stage + lane * pass_dims * wide;
+#pragma unroll
+                    for (int u = 0; u < 4; u++) {
+                        // positions of elements 0..7 within a unit of value codes
+                        constexpr int i8[8] = {0, 1, 2, 3, 4, 5, 6, 7}, i4[8] = {0, 2, 4, 6, 1, 3, 5, 7};
+                        const float f = split_part ? unit : unit * inv;
+                        float v[8];
+#pragma unroll
+                        for (int e = 0; e < 8; e++) v[e] = (o[8 * u + (BV == 8 ? i8[e] : i4[e])] + z) * f;
+                        const int ch = (d0 - p0 + 8 * u) * wide / 16;
+                        if (SPLIT || split_part) {
+                            sts4(row + ((ch ^ (lane & swz)) << 4), __float_as_uint(v[0]), __float_as_uint(v[1]),
                                  __float_as_uint(v[2]), __float_as_uint(v[3]));
-                            sts4(row + (((ch + 1) ^ (lane & SWZ)) << 4), __float_as_uint(v[4]), __float_as_uint(v[5]),
+                            sts4(row + (((ch + 1) ^ (lane & swz)) << 4), __float_as_uint(v[4]), __float_as_uint(v[5]),
                                  __float_as_uint(v[6]), __float_as_uint(v[7]));
                         } else {
-                            sts4(row + ((ch ^ (lane & SWZ)) << 4), pack16(v[0], v[1], p.out.fmt), pack16(v[2], v[3], p.out.fmt),
+                            sts4(row + ((ch ^ (lane & swz)) << 4), pack16(v[0], v[1], p.out.fmt), pack16(v[2], v[3], p.out.fmt),
                                  pack16(v[4], v[5], p.out.fmt), pack16(v[6], v[7], p.out.fmt));
                         }
                     }
                 }
-            }
-            if (!rec) {
                 __syncwarp();
-                constexpr int RPI = 32 / CPR;  // rows of one store
 #pragma unroll 4
-                for (int it = 0; it < CPR; it++) {
-                    const int rr = it * RPI + lane / CPR, ch = lane % CPR;
-                    const float4 v = lds4(stage + rr * ROWB + ((ch ^ (rr & SWZ)) << 4));
+                for (int id = lane; id < 32 * cpr; id += 32) {
+                    const int rr = id / cpr, ch = id % cpr;  // (cpr is a power of two)
+                    const float4 v = lds4(stage + rr * (pass_dims * wide) + ((ch ^ (rr & swz)) << 4));
                     const uint32_t tile_row = (uint32_t)(base_row + rr), gr = rows.r0 + tile_row;
-                    const uint32_t tok = kv_div(gr, p.group_magic);
-                    if (tile_row < rows.n)
+                    if (tile_row >= rows.n) continue;
+                    if (split_part) {
+                        *reinterpret_cast<float4 *>(p.part + record(tile_row) * D + p0 + ch * 4) = v;
+                    } else {
+                        const uint32_t tok = kv_div(gr, p.group_magic);
                         *reinterpret_cast<float4 *>(static_cast<uint8_t *>(p.out.data) +
                                                     ((size_t)(seq.q0 + tok) * p.out.row_stride +
                                                      (h * G + gr - tok * G) * p.out.head_stride) * ES + ch * 16) = v;
+                    }
                 }
             }
-            if (rec && valid) *reinterpret_cast<float2 *>(rec + D) = make_float2(l == 0.0f ? -INFINITY : row_ref[in_tile], l);
+            if (split_part && valid)
+                reinterpret_cast<float2 *>(p.ml)[record(in_tile)] = make_float2(l == 0.0f ? -INFINITY : row_ref[in_tile], l);
         }
     } else if (warp < 12) {
         // ================= producers: codes to f16 operands =================

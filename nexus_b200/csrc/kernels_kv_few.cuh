@@ -167,7 +167,7 @@ __device__ __forceinline__ void join(float &m, float &l, float (&v)[8], float m1
 #pragma unroll
     for (int j = 0; j < 8; j++) v[j] = fmaf(v1[j], f1, v[j] * f);
 }
-// Record of row r of a (sequence, KV head) pair and split s: D floats o, then m, l.
+// Record of row r of a (sequence, KV head) pair and split s.
 __host__ __device__ inline size_t few_record(uint32_t pair, uint32_t rows, uint32_t r, uint32_t nsplit, uint32_t s) {
     return ((size_t)pair * rows + r) * nsplit + s;
 }
@@ -678,10 +678,12 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? (SPLIT ? 3 : 4) : 2) k_
             join(top, l_all, v, src[D], src[D + 1], v1);
         }
         if (p.nsplit > 1) {
-            float *dst = p.cluster ? mine + r * RS : p.part + few_record(pair, R, r, p.nsplit, split) * RS;
+            const size_t at = few_record(pair, R, r, p.nsplit, split);
+            float *dst = p.cluster ? mine + r * RS : p.part + at * D;
+            float *ml = p.cluster ? mine + r * RS + D : p.ml + at * 2;
 #pragma unroll
             for (int j = 0; j < 8; j += 2) *reinterpret_cast<float2 *>(dst + d0 + j) = make_float2(v[j], v[j + 1]);
-            if (d0 == 0) *reinterpret_cast<float2 *>(dst + D) = make_float2(top, l_all);
+            if (d0 == 0) *reinterpret_cast<float2 *>(ml) = make_float2(top, l_all);
         } else {
             finish(r, d0, l_all, v);
         }

@@ -123,6 +123,7 @@ int cuda_fail(nexus_cuda_backend *b, cudaError_t e) {
 // sizes and bounds, so that the workspace query and a captured call agree.
 struct Split {
     uint32_t tile_rows, row_tiles, nsplit, tiles_per_split;
+    size_t records;  // of the workspace, each D + 2 floats
     size_t bytes;
 };
 struct AttnPlan {
@@ -134,9 +135,10 @@ struct AttnPlan {
     size_t bytes;
 };
 
-size_t part_bytes(const Split &s, uint64_t tiles, uint32_t head_dim) {
-    if (s.nsplit <= 1) return 0;
-    return ((size_t)tiles * s.tile_rows * s.nsplit * (head_dim + 2) * sizeof(float) + 15) & ~(size_t)15;
+void plan_records(Split *s, uint64_t tiles, uint32_t head_dim) {
+    if (s->nsplit <= 1) return;
+    s->records = (size_t)tiles * s->tile_rows * s->nsplit;
+    s->bytes = s->records * (head_dim + 2) * sizeof(float);  // (tile_rows is even: a multiple of 16)
 }
 
 const char *attn_plan(const nexus_kv_cache *c, const nexus_kv_batch *t, const nexus_kv_rows *q, uint32_t window,
@@ -168,15 +170,15 @@ const char *attn_plan(const nexus_kv_cache *c, const nexus_kv_batch *t, const ne
         // every CTA is resident at once (64 ragged sequences: 154 us so, 117 with the
         // workspace).
         pl->cluster = pl->f.nsplit <= kKvCluster && ctas * pl->f.nsplit <= kKvSms * 4;
-        if (!pl->cluster) pl->f.bytes = part_bytes(pl->f, ctas, c->head_dim);
+        if (!pl->cluster) plan_records(&pl->f, ctas, c->head_dim);
     }
     if (pl->chunk) {
         pl->c.tile_rows = kKvChunkRows;
         const uint64_t row_tiles = (rows + kKvChunkRows - 1) / kKvChunkRows;
         const uint32_t toks = t->max_q < kKvChunkRows ? t->max_q : kKvChunkRows;
         const uint32_t tiles = kv_tiles_bound(toks, t->max_kv, window, sinks, kKvChunkTile);
-        // one CTA an SM: parts only where the rows leave SMs without work, none
-        // shorter than four key tiles
+        // One CTA an SM: parts only where the rows leave SMs without work, none shorter
+        // than four key tiles.
         const uint64_t ctas = pairs * row_tiles, want = ctas >= kKvSms ? 1 : kKvSms / ctas;
         uint64_t per = (tiles + want - 1) / want;
         if (per < 4) per = 4;
@@ -184,7 +186,7 @@ const char *attn_plan(const nexus_kv_cache *c, const nexus_kv_batch *t, const ne
         pl->c.nsplit = tiles ? (uint32_t)((tiles + per - 1) / per) : 1;
         if (row_tiles * pl->c.nsplit > 65535) return "kv attention: too many rows per sequence for one call";
         pl->c.row_tiles = (uint32_t)row_tiles;
-        pl->c.bytes = part_bytes(pl->c, ctas, c->head_dim);
+        plan_records(&pl->c, ctas, c->head_dim);
         if (q->format == NEXUS_FMT_F32 && per > kKvFlushTiles)
             pl->sums = (size_t)ctas * pl->c.nsplit * kKvChunkRows * c->head_dim * sizeof(float);
     }
@@ -306,6 +308,7 @@ extern "C" int nexus_cuda_kv_attention(nexus_cuda_backend *b, const nexus_kv_cac
         p.cluster = !chunk && pl.cluster;
         uint8_t *ws = static_cast<uint8_t *>(workspace);
         p.part = reinterpret_cast<float *>(ws + (chunk ? pl.f.bytes : 0));
+        p.ml = p.part + s.records * cache->head_dim;
         p.sums = reinterpret_cast<float *>(ws + pl.f.bytes + pl.c.bytes);
         if (r == cudaSuccess) r = chunk ? launch_kv_attn_chunk(p, st) : launch_kv_attn_few(p, st);
         if (r == cudaSuccess && p.nsplit > 1 && !p.cluster) r = launch_kv_merge(p, st);
