@@ -2,8 +2,9 @@
 // draft window) over the quantised paged KV cache.
 //
 // For one (sequence, KV head) the rows are the new tokens x the G query heads
-// of the group (row r: token r / G, head r % G of the group), in tiles of 8 or 16.  With key j = zk_j + sk_j * kc_j (kc integer codes
-// around zero, zk = 0 for 8 bits) and likewise values:
+// of the group (row r: token r / G, head r % G of the group), in tiles of 8 or
+// 16.  With key j = zk_j + sk_j * kc_j (kc integer codes around zero, zk = 0 for
+// 8 bits) and likewise values:
 //   x_rj = c_r * (sk_j * (q_r . kc_j) + zk_j * sum(q_r)),  p = 2^(x - m_r)
 //   o_r  = ( sum_j (p sv_j) vc_j + sum_j p zv_j ) / sum_j p
 // so the two products run on exact small integers in f16 and everything that
@@ -27,9 +28,14 @@
 //  - A warp owns 16-token tiles (one page holds a tile whole); their codes and
 //    scales come by cp.async into a ring of three slots of its own, so two tiles a
 //    warp are in flight and no barrier is in the loop.
-//  - The context is split over CTAs.  Up to eight parts are a cluster, which joins
-//    them through distributed shared memory (parts beyond a sequence's end leave at
-//    once); more go to the workspace and k_kv_merge joins them.  Either way in order.
+//  - The context is split over CTAs.  Up to eight parts, where every CTA of the call
+//    is resident at once, are a cluster, which joins them through distributed shared
+//    memory (parts beyond a sequence's end leave at once); otherwise they go to the
+//    workspace and k_kv_merge joins them.  Either way in order.
+// Measured: 64 sequences of 1024 to 8192 tokens, 32/8 heads, bf16: 114 us at 4 bits
+// (3.0 TB/s; bound by the instructions that unpack and the latencies of a tile's
+// chain), 133 us at 8 bits (4.7 TB/s); one of 131071 tokens, 64/8 heads, 8 bits:
+// 54 us (5.1 TB/s) and 14 us of joining.
 #pragma once
 #include <type_traits>
 
@@ -690,6 +696,7 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? (SPLIT ? 3 : 4) : 2) k_
     }
     if (p.cluster && p.nsplit > 1) {
         const uint32_t used = max(1u, (tiles.total + p.tiles_per_split - 1) / p.tiles_per_split);
+        __syncwarp();
         cluster_sync();
         for (uint32_t i = split * (kWarps * 32) + threadIdx.x; i < rows.n * (D / 8); i += used * (kWarps * 32)) {
             const uint32_t r = i / (D / 8), d0 = (i % (D / 8)) * 8;
@@ -703,6 +710,7 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? (SPLIT ? 3 : 4) : 2) k_
             }
             finish(r, d0, l_all, v);
         }
+        __syncwarp();
         cluster_sync();  // nobody leaves while its records are read
     }
 }

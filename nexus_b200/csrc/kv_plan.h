@@ -126,6 +126,13 @@ NX_HD KvRowTile kv_row_tile(const KvSeqView &s, uint32_t G, uint32_t rt, uint32_
     return t;
 }
 
+// A number of its own for row tile rt of every sequence, below rows * G / R +
+// n_seqs for a batch of `rows` rows: floor((x + y)) + 1 >= floor(x) + ceil(y), so
+// the next sequence's numbers start behind this one's.
+NX_HD uint64_t kv_tile_slot(uint32_t q0, uint32_t G, uint32_t b, uint32_t rt, uint32_t R) {
+    return (uint64_t)q0 * G / R + b + rt;
+}
+
 // An upper bound of kv_tiles().total for nq <= q queries of a sequence of at
 // most max_kv tokens.
 NX_HD uint32_t kv_tiles_bound(uint32_t q, uint32_t max_kv, uint32_t window, uint32_t sinks, uint32_t T) {

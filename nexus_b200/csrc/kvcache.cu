@@ -188,7 +188,8 @@ const char *attn_plan(const nexus_kv_cache *c, const nexus_kv_batch *t, const ne
         pl->c.row_tiles = (uint32_t)row_tiles;
         plan_records(&pl->c, ctas, c->head_dim);
         if (q->format == NEXUS_FMT_F32 && per > kKvFlushTiles)
-            pl->sums = (size_t)ctas * pl->c.nsplit * kKvChunkRows * c->head_dim * sizeof(float);
+            pl->sums = (size_t)(((uint64_t)q->rows * G / kKvChunkRows + t->n_seqs) * c->kv_heads) * pl->c.nsplit *
+                       kKvChunkRows * c->head_dim * sizeof(float);  // (kv_tile_slot)
     }
     pl->bytes = pl->f.bytes + pl->c.bytes + pl->sums;
     return nullptr;

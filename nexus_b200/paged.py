@@ -187,7 +187,7 @@ class PagedKvCache:
             out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
         bt, rq, ro = self._batch(batch), self._rows(q, "q"), self._rows(out, "out")
         qr = C.byref(rq)
-        key = (rq.heads, rq.format, rq.rows > 0, window, sinks, self._shape)
+        key = (rq.heads, rq.format, rq.rows, window, sinks, self._shape)
         need = batch._workspaces.get(key)
         if need is None:
             size = C.c_size_t()

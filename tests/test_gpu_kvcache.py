@@ -441,6 +441,52 @@ def test_f32_stays_exact_over_long_contexts(backend, nb, new, dim, bits):
         assert float((out[rows].double() - ref).norm() / ref.norm()) < 2e-6
 
 
+@pytest.mark.parametrize("new", [1, 60])
+def test_cache_beyond_32_bit_offsets(backend, nb, new):
+    """Pages whose codes lie beyond 4 GB of the pool, written, read and attended."""
+    pages = (1 << 32) // (8 * 16 * 128) + 2000
+    cache = nb.PagedKvCache.empty(backend, pages, 8, 128, 16, (8, 8))
+    lens = [(new, 150), (new, max(new, 33))]
+    table = torch.stack([torch.arange(pages - 1, pages - 13, -1), torch.arange(pages - 20, pages - 32, -1)]).to(torch.int32)
+    for b in range(2):
+        ids = table[b].long().to(DEV)
+        for codes, scales in ((cache.k_codes, cache.k_scales), (cache.v_codes, cache.v_scales)):
+            codes[ids] = torch.randint(0, 256, codes[ids].shape, generator=gen(60 + b), device=DEV, dtype=torch.uint8)
+            scales[ids] = 0.02
+    batch = nb.KvBatch(torch.tensor([0, new, 2 * new], dtype=torch.int32, device=DEV),
+                       torch.tensor([kv for _, kv in lens], dtype=torch.int32, device=DEV), table.to(DEV), new, 150)
+    x = torch.randn((2 * new, 48, 128), generator=gen(62), device=DEV).bfloat16()
+    cache.append(batch, x[:, 32:40], x[:, 40:])
+    k, _ = cache.read(batch, 2 * new)
+    assert torch.equal(k, R.held(*R.quantise(x[:, 32:40], 8), 8).float())
+    check_attention(cache, batch, lens, x[:, :32])
+    assert not cache.k_codes[: pages - 40].any()
+
+
+def test_nothing_to_do(backend, nb):
+    """No sequences, no rows, sequences without new tokens."""
+    cache = nb.PagedKvCache.empty(backend, 4, 2, 64)
+    none = torch.zeros((0, 2, 64), device=DEV)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    for batch in (nb.KvBatch(i32(0), i32(), torch.zeros((0, 3), dtype=torch.int32, device=DEV), 0, 0),
+                  nb.KvBatch(i32(0, 0, 0), i32(5, 0), torch.zeros((2, 3), dtype=torch.int32, device=DEV), 0, 5)):
+        cache.append(batch, none, none)
+        assert cache.read(batch, 0)[0].shape == (0, 2, 64)
+        assert cache.attention(batch, torch.zeros((0, 4, 64), device=DEV)).shape == (0, 4, 64)
+        rows = torch.full((3, 4, 64), 2.0, device=DEV)
+        assert bool((cache.attention(batch, rows, out=rows.clone()) == 2.0).all())
+    cache.status()
+
+
+def test_one_long_chunk_among_single_tokens_f32(backend, nb):
+    lens = [(1, 900)] * 5 + [(700, 1500)] + [(1, 40)] * 5 + [(33, 2000)]
+    batch, pages, rows = make_batch(nb, lens, 16)
+    cache = nb.PagedKvCache.empty(backend, pages, 2, 64, 16, (8, 8))
+    fill_random(cache, 63)
+    q = torch.randn((rows, 8, 64), generator=gen(64), device=DEV)
+    check_attention(cache, batch, lens, q)
+
+
 # ---------------------------------------------------------------- used together
 
 @pytest.mark.parametrize("bits", [(8, 8), (4, 4)])

@@ -112,6 +112,15 @@ def test_bad_copies_are_refused(nb):
     assert "unknown flag" in message(nb, lib.nexus_cuda_kv_status(None, None, 4))
 
 
+def test_workspace_of_f32_chunks_follows_the_rows(nb):
+    """One long chunk among many single tokens: the sums take the rows that are there, not n_seqs * max_q."""
+    lib, n = nb._lib.load(), C.c_size_t()
+    t = batch(nb, n_seqs=64, max_q=8192, max_kv=9000, table_stride=600)
+    q = rows(nb, 32, rows=8192 + 63, format=nb.F32)
+    assert lib.nexus_cuda_kv_attention_workspace(C.byref(cache(nb)), C.byref(t), C.byref(q), 0, 0, C.byref(n)) == 0
+    assert n.value < (8192 + 63 + 64 * 64) * 32 * 128 * 4 * 2
+
+
 def test_workspace_follows_sizes_only(nb):
     lib = nb._lib.load()
 
@@ -208,6 +217,22 @@ int main() {
         }
         CHECK(rows == nq * G);
         if (nq * G) CHECK(kv_row_tile(s, G, 0, R, nq * G - 1).n == 0);
+    }
+    // tile slots: one for each (sequence, row tile), below the bound
+    for (int rep = 0; rep < 2000; rep++) {
+        const uint32_t G = 1 + std::rand() % 128, n = 1 + std::rand() % 9;
+        uint64_t at = 0;
+        uint32_t q0 = std::rand() % 50;
+        for (uint32_t b = 0; b < n; b++) {
+            const uint32_t nq = std::rand() % 3 ? std::rand() % 40 : std::rand() % 4000;
+            for (uint32_t rt = 0; (uint64_t)rt * 256 < (uint64_t)nq * G; rt++) {
+                const uint64_t slot = kv_tile_slot(q0, G, b, rt, 256);
+                CHECK(slot >= at);
+                at = slot + 1;
+            }
+            q0 += nq;
+        }
+        CHECK(at <= (uint64_t)q0 * G / 256 + n);
     }
     return 0;
 }
