@@ -38,7 +38,7 @@ struct KvAttnParams {
     KvCacheView cache;
     KvBatchView batch;
     KvRows q, out;
-    int hq, group;
+    int group;
     uint32_t group_magic;      // ceil(2^32 / group), 0 for a group of one (kv_div)
     float scale_log2;          // score scale * log2(e)
     uint32_t window, sinks;

@@ -955,7 +955,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
         // ================= MMA issue (whole warp, elected lane) =================
         // One warp for both row tiles, in turn: each tile's products run while the
         // other's softmax does (with a warp each, the two fell into step and the
-        // tensor pipe waited: 5.2 against 4.8 us a key tile).  The products run in
+        // tensor pipe waited: 2048 tokens behind 14336 took 1020 against 979 us).  The products run in
         // the order of issue: P V reads P before the next S is written over it.
         constexpr uint32_t id_s = idesc_f16(kTok, false), id_o = idesc_f16(D, true);
         const uint32_t q0 = sbase, k0 = sbase + S::K0, v0 = sbase + S::V0;

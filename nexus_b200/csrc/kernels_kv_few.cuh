@@ -34,8 +34,8 @@
 //    workspace and k_kv_merge joins them.  Either way in order.
 // Measured: 64 sequences of 1024 to 8192 tokens, 32/8 heads, bf16: 114 us at 4 bits
 // (3.0 TB/s; bound by the instructions that unpack and the latencies of a tile's
-// chain), 133 us at 8 bits (4.7 TB/s); one of 131071 tokens, 64/8 heads, 8 bits:
-// 54 us (5.1 TB/s) and 14 us of joining.
+// chain), 133 us at 8 bits (4.7 TB/s); one of 131071 tokens, 64/8 heads, f16, 8 bits:
+// 59 us with its join (4.7 TB/s).
 #pragma once
 #include <type_traits>
 
@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? (SPLIT ? 3 : 4) : 2) k_
     extern __shared__ __align__(128) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     constexpr uint32_t R = 8 * NR;
-    const uint32_t split = blockIdx.x % p.nsplit, rt = blockIdx.x / p.nsplit, h = blockIdx.y, b = blockIdx.z;
+    const uint32_t split = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
     unsigned fault = 0;
     const KvSeqView seq = kv_load_seq(p.batch, b, p.cache.shift, &fault);
     if (fault) {
@@ -197,7 +197,7 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? (SPLIT ? 3 : 4) : 2) k_
         return;
     }
     const uint32_t G = (uint32_t)p.group;
-    const KvRowTile rows = kv_row_tile(seq, G, rt, R, p.rows_limit);
+    const KvRowTile rows = kv_row_tile(seq, G, 0, R, p.rows_limit);
     if (rows.n == 0) return;
     const int pos0 = (int)seq.kv - (int)seq.nq;
     const KvRange range = kv_range(rows.first, rows.last, p.window, p.sinks);
@@ -663,7 +663,7 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? (SPLIT ? 3 : 4) : 2) k_
             }
         }
     __syncthreads();
-    const uint32_t pair = (b * p.cache.hkv + h) * p.row_tiles + rt;
+    const uint32_t pair = b * p.cache.hkv + h;
     float *mine = rec + kWarps * 8 * NR * RS;  // this part's records, for the cluster
     auto finish = [&](uint32_t r, uint32_t d0, float l_all, float(&v)[8]) {
         const float inv = l_all == 0.0f ? 0.0f : 1.0f / l_all;
@@ -726,7 +726,7 @@ cudaError_t launch_few_t(const KvAttnParams &p, cudaStream_t st) {
         if (e != cudaSuccess) return e;
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(p.nsplit * p.row_tiles, p.cache.hkv, p.batch.n_seqs);
+    cfg.gridDim = dim3(p.nsplit, p.cache.hkv, p.batch.n_seqs);
     cfg.blockDim = dim3(kWarps * 32);
     cfg.dynamicSmemBytes = SMEM;
     cfg.stream = st;

@@ -154,22 +154,32 @@ const char *attn_plan(const nexus_kv_cache *c, const nexus_kv_batch *t, const ne
     if (pl->few) {
         const uint32_t most = rows < kKvFewRows ? (uint32_t)rows : kKvFewRows;
         pl->f.tile_rows = most <= 8 ? 8 : 16;
-        pl->f.row_tiles = (most + pl->f.tile_rows - 1) / pl->f.tile_rows;
+        pl->f.row_tiles = 1;
         const uint32_t tiles = kv_tiles_bound((most + G - 1) / G, t->max_kv, window, sinks, kKvFewTile);
-        // Parts of 8 to 64 tiles, three CTAs an SM or more while they are short, and no
-        // more than 32 CTAs an SM in all.  Measured (us): one sequence of 577 tokens 14.3
-        // with 8 tiles, 16.4 with 16; of 16000 tokens 24.6 with 27 or 32, 32.8 with 8; 64
-        // sequences of 1024 to 8192 tokens 117 with 64, 139 with 256.
-        const uint64_t ctas = pairs * pl->f.row_tiles, all = (uint64_t)tiles * ctas;
+        // CTAs resident at once, by the registers of the variant (kernels_kv_few.cuh).
+        const uint64_t slots = kKvSms * (pl->f.tile_rows == 16 ? 2 : q->format == NEXUS_FMT_F32 ? 3 : 4);
+        // Parts of 8 to 64 tiles, three CTAs an SM while they are short and at most 32 an
+        // SM in all.  Few long sequences, and what would be a little more than one round
+        // of CTAs, take one round.  Measured (us): one sequence of 577 tokens 14.3 with 8
+        // tiles, 16.4 with 16; of 16000 tokens 24.6 with 27 or 32, 32.8 with 8; of 131071
+        // tokens (64/8 heads) 59 in one round of 74 parts, 67 in 128; 64 sequences of 1024
+        // to 8192 tokens 117 with 64 tiles, 139 with 256.
+        const uint64_t ctas = pairs, all = (uint64_t)tiles * ctas;
         uint64_t per = (all + kKvSms * 3 - 1) / (kKvSms * 3);
         per = per < 8 ? 8 : per > 64 ? 64 : per;
+        if (ctas * 2 <= kKvSms && per == 64) per = (all + slots - 1) / slots;
         if (per < (all + kKvSms * 32 - 1) / (kKvSms * 32)) per = (all + kKvSms * 32 - 1) / (kKvSms * 32);
+        uint64_t nsplit = tiles ? (tiles + per - 1) / per : 1;
+        if (ctas <= slots && ctas * nsplit > slots && ctas * nsplit < 2 * slots) {
+            per = (tiles + slots / ctas - 1) / (slots / ctas);
+            nsplit = (tiles + per - 1) / per;
+        }
         pl->f.tiles_per_split = (uint32_t)per;
-        pl->f.nsplit = tiles ? (uint32_t)((tiles + per - 1) / per) : 1;
+        pl->f.nsplit = (uint32_t)nsplit;
         // A cluster's parts wait for one another and hold their SM meanwhile: only where
         // every CTA is resident at once (64 ragged sequences: 154 us so, 117 with the
         // workspace).
-        pl->cluster = pl->f.nsplit <= kKvCluster && ctas * pl->f.nsplit <= kKvSms * 4;
+        pl->cluster = nsplit <= kKvCluster && ctas * nsplit <= slots;
         if (!pl->cluster) plan_records(&pl->f, ctas, c->head_dim);
     }
     if (pl->chunk) {
@@ -289,7 +299,6 @@ extern "C" int nexus_cuda_kv_attention(nexus_cuda_backend *b, const nexus_kv_cac
     p.batch = batch_view(batch, q->rows);
     p.q = rows_view(q);
     p.out = rows_view(out);
-    p.hq = (int)q->heads;
     p.group = (int)(q->heads / cache->kv_heads);
     p.group_magic = kv_div_magic((uint32_t)p.group);
     p.scale_log2 = (scale != 0.0f ? scale : 1.0f / sqrtf((float)cache->head_dim)) * 1.4426950408889634f;
