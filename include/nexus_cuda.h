@@ -535,8 +535,9 @@ int nexus_cuda_kv_read(nexus_cuda_backend *b, const nexus_kv_cache *cache, const
 /* Causal GQA attention of the batch's query rows over the cache, which holds
  * their own tokens already: the query at position i sees key j when j <= i and
  * (window == 0 or j > i - window or j < sinks).  Query head q uses KV head
- * q / (q heads / kv heads); at most 128 query heads per KV head.  scale 0
- * means 1/sqrt(head_dim).  out has q's format and heads.  The workspace
+ * q / (q heads / kv heads); at most 128 query heads per KV head.  scale is
+ * at most 2e38, 0 means 1/sqrt(head_dim).  out has q's format and heads; it may
+ * be q itself (same data and strides), but must not overlap it otherwise.  The workspace
  * (device, 16-byte aligned, contents free before and after) holds at least
  * nexus_cuda_kv_attention_workspace bytes and belongs to this call until it
  * has run: calls that may overlap need one each. */

@@ -280,7 +280,8 @@ extern "C" int nexus_cuda_kv_attention(nexus_cuda_backend *b, const nexus_kv_cac
     if (!e) e = check_rows(out, cache->head_dim, true);
     if (!e && (out->rows != q->rows || out->heads != q->heads || out->format != q->format))
         e = "kv attention: out must have q's rows, heads and format";
-    if (!e && !(scale >= 0.0f && scale <= 3.0e38f)) e = "kv attention: scale must be finite and not negative";
+    // (the kernels take it times log2(e), which has to stay in f32)
+    if (!e && !(scale >= 0.0f && scale <= 2.0e38f)) e = "kv attention: scale must be in [0, 2e38]";
     AttnPlan pl;
     if (!e) e = attn_plan(cache, batch, q, window, sinks, &pl);
     if (!e && pl.bytes && (!workspace || workspace_bytes < pl.bytes)) e = "kv attention: workspace too small";

@@ -179,10 +179,13 @@ class PagedKvCache:
                   sinks: int = 0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Causal GQA attention of q ([rows, heads, head_dim]) over the cached
         tokens, the rows' own among them; with a window, key j is visible to
-        position i when j > i - window or j < sinks.  Rows outside every
-        sequence are left as they were (undefined without `out`)."""
+        position i when j > i - window or j < sinks.  `scale` (default
+        1/sqrt(head_dim)) is positive; `out` may be q itself.  Rows outside
+        every sequence are left as they were (undefined without `out`)."""
         if window < 0 or sinks < 0:
             raise _invalid("window and sinks must not be negative")
+        if scale is not None and not scale > 1e-45:  # 0 in f32 would ask for the default
+            raise _invalid("scale must be positive")
         if out is None:
             out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
         bt, rq, ro = self._batch(batch), self._rows(q, "q"), self._rows(out, "out")

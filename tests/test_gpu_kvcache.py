@@ -403,6 +403,22 @@ def test_score_scale(backend, nb):
         check_attention(cache, batch, lens, q, scale=s)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lens", [[(1, 90), (1, 40)], [(1, 9000)] * 2, [(1, 90000)], [(2, 300), (70, 200), (300, 800)],
+                                  [(40, 6000)], [(0, 0), (5, 3), (1, 1)]])
+def test_output_in_place_of_the_queries(backend, nb, lens, dtype):
+    """One part, parts of a cluster, parts in the workspace, and chunks of one part and of several."""
+    batch, pages, rows = make_batch(nb, lens, 16)
+    cache = nb.PagedKvCache.empty(backend, pages, 2, 64, 16, (8, 4))
+    fill_random(cache, 37)
+    q = torch.randn((rows, 8, 64), generator=gen(38), device=DEV).to(DTYPES[dtype])
+    want = cache.attention(batch, q)
+    got = q.clone()
+    cache.attention(batch, got, out=got)
+    cache.status()
+    assert torch.equal(got.view(torch.uint8), want.view(torch.uint8))
+
+
 def test_same_call_same_bits(backend, nb):
     lens = [(1, 5000), (60, 3000), (2, 900)]
     batch, pages, rows = make_batch(nb, lens, 16)

@@ -247,3 +247,17 @@ def test_index_arithmetic(tmp_path):
                     f"-I{ROOT / 'nexus_b200' / 'csrc'}", str(src), "-o", str(exe)], check=True)
     r = subprocess.run([str(exe)], capture_output=True, text=True)
     assert r.returncode == 0, r.stdout + r.stderr
+
+
+def test_score_scale_keeps_its_product_in_f32(nb):
+    """2.5e38 * log2(e) is beyond f32, 2e38 * log2(e) is not."""
+    assert "scale" in attention(nb, scale=2.5e38)
+    assert "backend" in attention(nb, scale=2e38)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.0, -1.0, 1e-50, float("nan")])
+def test_binding_refuses_a_scale_that_is_not_positive(nb, scale):
+    """0 asks the C call for its default, so a caller's own 0 must not reach it."""
+    c = nb.PagedKvCache.__new__(nb.PagedKvCache)
+    with pytest.raises(nb.NexusError, match="scale"):
+        c.attention(None, None, scale=scale)
