@@ -986,7 +986,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
                 if constexpr (SPLIT) umma_f16_ts_w(tmem + kOCol + D * sub, a + 8, bd, id_o, 1);
             }
         };
-        if (n > 0 && wait(&qfull, 0) && wait(&kfull[0], 0)) {
+        // (also without a key tile: the outputs are staged where the queries are being converted)
+        if (wait(&qfull, 0) && n > 0 && wait(&kfull[0], 0)) {
             for (int sub = 0; sub < 2; sub++)
                 if (active(sub, 0)) mma_s(sub, 0);
             umma_commit_w(&kempty[0]);
