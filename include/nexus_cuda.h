@@ -501,7 +501,8 @@ typedef struct {
     uint32_t n_seqs;
     uint32_t max_q;         /* most new tokens of any sequence */
     uint32_t max_kv;        /* longest kv_len */
-    uint32_t table_stride;  /* page table entries per sequence */
+    uint32_t table_stride;  /* page table entries from one sequence to the next; max_kv tells how many
+                               of them a sequence may use where that is fewer */
     const uint32_t *q_start, *kv_len, *page_table; /* device */
     void *stream;           /* cudaStream_t the call runs on, with NEXUS_KV_CALLER_STREAM */
     uint32_t flags;

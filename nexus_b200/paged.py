@@ -44,7 +44,8 @@ class KvBatch:
     """A ragged batch: sequence b brings rows q_start[b]..q_start[b + 1] of the
     row tensors, the last of its kv_len[b] tokens; token t lives in page
     page_table[b, t // page_tokens].  int32 CUDA tensors (kept by reference);
-    max_q and max_kv bound the new tokens and the length of any sequence."""
+    max_q and max_kv bound the new tokens and the length of any sequence, as
+    the columns of page_table (which may be a slice of a wider table) do."""
 
     def __init__(self, q_start: torch.Tensor, kv_len: torch.Tensor, page_table: torch.Tensor, max_q: int,
                  max_kv: int):
@@ -69,16 +70,20 @@ class KvBatch:
             raise _invalid("max_q and max_kv must be in [0, 2^31)")
         self.q_start, self.kv_len, self.page_table = q_start, kv_len, page_table
         self.max_q, self.max_kv = int(max_q), int(max_kv)
-        self._args = (n, self.max_q, self.max_kv, page_table.stride(0) if n > 1 else page_table.shape[1],
-                      q_start.data_ptr(), kv_len.data_ptr(), page_table.data_ptr())
+        self._args = (page_table.stride(0) if n > 1 else page_table.shape[1], q_start.data_ptr(), kv_len.data_ptr(),
+                      page_table.data_ptr())
         self._index = kv_len.get_device()
-        self._structs = {}     # by stream: filled once, never changed
+        self._structs = {}     # by stream and page size: filled once, never changed
         self._workspaces = {}  # bytes by what they depend on
 
-    def _ref(self, stream: int):
-        r = self._structs.get(stream)
+    def _ref(self, stream: int, page_tokens: int):
+        r = self._structs.get((stream, page_tokens))
         if r is None:
-            r = self._structs[stream] = C.byref(L.KvBatch(*self._args, stream, L.KV_CALLER_STREAM))
+            # the rows of a table that is a slice of a wider one are further apart than they
+            # have entries: a sequence ends with its entries, not with the row's pitch
+            max_kv = min(self.max_kv, self.page_table.shape[1] * page_tokens)
+            r = self._structs[stream, page_tokens] = C.byref(
+                L.KvBatch(self.kv_len.numel(), self.max_q, max_kv, *self._args, stream, L.KV_CALLER_STREAM))
         return r
 
 
@@ -132,7 +137,7 @@ class PagedKvCache:
     def _batch(self, batch: KvBatch):
         if batch._index != self.backend.device:
             raise _invalid(f"the batch is on cuda:{batch._index}, the backend on {self.device}")
-        return batch._ref(_raw_stream(self.backend.device))
+        return batch._ref(_raw_stream(self.backend.device), self.page_tokens)
 
     def _rows(self, t: torch.Tensor, what: str) -> L.KvRows:
         fmt = _FORMATS.get(t.dtype)

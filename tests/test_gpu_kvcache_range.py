@@ -28,3 +28,29 @@ def test_row_tiles_of_padding_alone(backend, nb, dim, dtype):
         cache.attention(batch, q, out=out)
     cache.status()
     assert all(torch.equal(out.double(), first) for out in outs)
+
+
+@pytest.mark.parametrize("new", [1, 60])
+def test_a_sliced_page_table_ends_with_its_columns(backend, nb, new):
+    """Columns of a wider table: a length beyond them is a fault, whatever stands behind them."""
+    wide = torch.full((2, 40), 5, dtype=torch.int32, device=DEV)
+    wide[:, 30:] = torch.randperm(20, generator=torch.Generator().manual_seed(2)).view(2, 10).to(torch.int32)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    cache = nb.PagedKvCache.empty(backend, 24, 2, 64)
+    fill_random(cache, 82)
+    lens = [(new, 160), (new, 150)]
+    batch = nb.KvBatch(i32(0, new, 2 * new), i32(160, 150), wide[:, 30:], new, 1000)
+    x = torch.randn((2 * new, 12, 64), generator=gen(83), device=DEV).half()
+    want = check_attention(cache, batch, lens, x[:, :8])
+    batch.kv_len[1] = 161
+    out = torch.zeros_like(x[:, :8])
+    cache.attention(batch, x[:, :8], out=out)
+    with pytest.raises(nb.NexusError, match="page table"):
+        cache.status()
+    assert torch.equal(out[:new].double(), want[:new]) and not out[new:].any()
+    before = cache.k_codes.clone()
+    cache.append(batch, x[:, 8:10], x[:, 10:])
+    with pytest.raises(nb.NexusError, match="page table"):
+        cache.status()
+    changed = (cache.k_codes != before).flatten(1).any(-1).nonzero().flatten().tolist()
+    assert set(changed) <= set(wide[0, 30:].tolist())

@@ -1,0 +1,26 @@
+"""The Python binding of the quantised paged KV cache without a GPU: what it hands to the C calls, and its refusals."""
+import pytest
+import torch
+
+
+class OnGpu(torch.Tensor):
+    """A CPU tensor that says it is on cuda:0 (no call here reaches a device)."""
+    is_cuda = property(lambda self: True)
+
+    def get_device(self):
+        return 0
+
+
+def i32(*shape):
+    return torch.zeros(shape, dtype=torch.int32).as_subclass(OnGpu)
+
+
+def test_a_slice_of_a_table_bounds_its_sequences(nb):
+    """Four columns of a table of sixteen: 64 tokens of 16 a sequence, not 256."""
+    table = torch.zeros((3, 16), dtype=torch.int32)[:, 12:].as_subclass(OnGpu)
+    batch = nb.KvBatch(i32(4), i32(3), table, 1, 200)
+    t = batch._ref(0, 16)._obj
+    assert (t.n_seqs, t.table_stride, t.max_kv) == (3, 16, 64)
+    assert batch._ref(0, 64)._obj.max_kv == 200  # pages of 64 tokens hold 256
+    assert batch._ref(0, 16)._obj.max_kv == 64
+    assert batch.max_kv == 200
