@@ -72,6 +72,7 @@ struct Slot {
     static constexpr int LV = 2048;            // log2 max(sv, |zv|)
     static constexpr int SMAX = 2560, ZMAX = 2576;  // largest sv, |zv| of each quarter of the tokens
     static constexpr int UNIT = 2592;          // what sv and zv were divided by
+    static constexpr int BAD = 2596;           // bit r: tokens 16 r .. of the tile have no page (nobody sees them)
     static constexpr int BYTES = 2608;
 };
 
@@ -440,7 +441,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
             if constexpr (SPLIT) {
                 if (cnt > 0 && cnt % kFlush == 0) flush(true);  // (the products before S have completed)
             }
-            const bool whole = j0 + kTok - 1 <= first &&
+            const uint32_t bad = __float_as_uint(lds1(sl + Slot::BAD));
+            const bool whole = bad == 0 && j0 + kTok - 1 <= first &&
                                (p.window == 0 || j0 > last - (int)p.window || j0 + kTok <= (int)p.sinks);
             unit = lds1(sl + Slot::UNIT);
             const float svmax = max4(lds4(sl + Slot::SMAX));
@@ -453,7 +455,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
             auto seen = [&](int k, int c0) {
                 const int hi = pos[k] - j0 + 1, lo = p.window ? max(0, pos[k] - (int)p.window + 1) - j0 : -1;
                 const int sink = min((int)min(p.sinks, 0x3fffffffu) - j0, hi);
-                return ((first_bits(hi - c0) & ~first_bits(lo - c0)) | first_bits(sink - c0)) >> (2 * c);
+                const uint32_t gone = (bad >> (c0 >> 4) & 1 ? 0xffffu : 0u) | (bad >> (c0 >> 4) & 2 ? 0xffff0000u : 0u);
+                return (((first_bits(hi - c0) & ~first_bits(lo - c0)) | first_bits(sink - c0)) & ~gone) >> (2 * c);
             };
             // the score of two columns in base 2, before the row's factor
             auto score = [&](const uint32_t *s, f2 sk, [[maybe_unused]] f2 zk, int k) {
@@ -777,11 +780,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
             const uint32_t j = tile_token(i) + 16 * lane;
             return kv_needed(range, j, j + 16) ? __ldg(table + (j >> p.cache.shift)) : ~0u;
         };
+        bool no_page = false;  // lane l < 8: run l of the tile is read and has no page in the pool
         auto page_ok = [&](uint32_t page, uint32_t i) -> uint32_t {
+            no_page = false;
             if (page < p.cache.num_pages) return page;
             if (i < n && lane < kTok / 16) {
                 const uint32_t j = tile_token(i) + 16 * lane;
-                if (kv_needed(range, j, j + 16)) fault = KV_FAULT_PAGE;
+                no_page = kv_needed(range, j, j + 16);
+                if (no_page) fault = KV_FAULT_PAGE;
             }
             return ~0u;
         };
@@ -790,8 +796,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
         };
         // A thread's chunks of 16 bytes: LC lanes a row, so that the eight lanes of
         // a store phase write eight different 16-byte columns of the swizzled rows
-        // Lane l < 8 finds run l; runs without a page read page 0 (their weights are
-        // zero whatever the codes), so that no load waits for a branch.
+        // Lane l < 8 finds run l; runs without a page read page 0 (nobody sees them), so
+        // that no load waits for a branch.
         auto load_codes = [&](auto bits_c, uint4 *dst, const uint8_t *codes, uint32_t pages, uint32_t i) {
             using C = Chunks<D, decltype(bits_c)::value>;
             const uint64_t run = reinterpret_cast<uint64_t>(codes) +
@@ -918,7 +924,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
                         sts1(sl + Slot::ZMAX + 4 * (pw + 2 * t), zm);
                     }
                 }
-                if (pt == 0) sts1(sl + Slot::UNIT, unit);
+                const uint32_t bad = __ballot_sync(0xffffffffu, no_page);
+                if (pt == 0) {
+                    sts1(sl + Slot::UNIT, unit);
+                    sts1(sl + Slot::BAD, __uint_as_float(bad));
+                }
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) {

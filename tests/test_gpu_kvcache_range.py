@@ -54,3 +54,31 @@ def test_a_sliced_page_table_ends_with_its_columns(backend, nb, new):
         cache.status()
     changed = (cache.k_codes != before).flatten(1).any(-1).nonzero().flatten().tolist()
     assert set(changed) <= set(wide[0, 30:].tolist())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("bits", [(8, 8), (4, 4)])
+@pytest.mark.parametrize("new", [1, 4, 60, 300])
+def test_tokens_of_a_page_beyond_the_pool_are_left_out(backend, nb, new, bits, dtype):
+    """One bad page among sound ones: what is left is the sequence without its tokens, in both
+    kernels.  The other scores are around -20 and below, so that a token counted with score 0
+    would take nearly all of the weight."""
+    kv, page, dim = new + 420, 16, 64
+    batch, pages, rows = make_batch(nb, [(new, kv)], page)
+    cache = nb.PagedKvCache.empty(backend, pages, 2, dim, page, bits)
+    fill_random(cache, 70)
+    q = (0.5 + torch.rand((rows, 8, dim), generator=gen(71), device=DEV)).to(DTYPES[dtype])
+    if bits[0] == 8:
+        cache.k_codes.copy_(cache.k_codes % 64)            # every element of a key below -0.02 * 64
+    else:
+        cache.k_scales[..., 1] = -2.0 - cache.k_scales[..., 1].abs()
+    for bad in (0, 9, 25):
+        whole = batch.page_table.clone()
+        batch.page_table[0, bad] = pages
+        out = cache.attention(batch, q)
+        with pytest.raises(nb.NexusError, match="page"):
+            cache.status()
+        batch.page_table.copy_(whole)
+        left = torch.cat([whole[:, :bad], whole[:, bad + 1:]], 1)
+        ref, spread, reach, floor = R.attention(q, cache, [(new, kv - page)], left)
+        assert bool(((out.double() - ref).abs() <= R.tolerance(ref, spread, reach, floor, q.dtype)).all())
