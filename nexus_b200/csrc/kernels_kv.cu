@@ -118,7 +118,12 @@ __device__ __forceinline__ void kv_quantise_group(float (&x)[8], uint8_t *codes,
             step *= kUp96;
             mid *= kUp96;
 #pragma unroll
-            for (int i = 0; i < 8; i++) x[i] *= kUp96;
+            for (int i = 0; i < 8; i++) {
+                x[i] *= kUp96;
+                // a subnormal scale can be rounded down by up to a third: quotients beyond 127
+                // (4-bit ones are clamped below, whatever the scale)
+                if constexpr (BITS == 8) x[i] = fminf(fmaxf(x[i], low * step), high * step);
+            }
         }
         const float inv = __fdividef(1.0f, step);
         float far = 0.0f;

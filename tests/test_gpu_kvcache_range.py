@@ -82,3 +82,21 @@ def test_tokens_of_a_page_beyond_the_pool_are_left_out(backend, nb, new, bits, d
         left = torch.cat([whole[:, :bad], whole[:, bad + 1:]], 1)
         ref, spread, reach, floor = R.attention(q, cache, [(new, kv - page)], left)
         assert bool(((out.double() - ref).abs() <= R.tolerance(ref, spread, reach, floor, q.dtype)).all())
+
+
+def test_append_subnormal_groups(backend, nb):
+    """f32 groups whose 8-bit scale is a few subnormal steps: its rounding takes quotients beyond
+    127, which are held as 127 (largest magnitudes 64 .. 17000 steps of 2^-149)."""
+    top = torch.arange(64, 17001, 7, device=DEV)
+    rows = top.numel()
+    batch, pages, n = make_batch(nb, [(rows, rows)], 64)
+    cache = nb.PagedKvCache.empty(backend, pages, 2, 64, 64, (8, 8))
+    steps = (torch.rand((rows, 2, 64), generator=gen(72), device=DEV) * 2 - 1) * top[:, None, None]
+    steps = steps.round().to(torch.int32)
+    steps[:, 0, 5], steps[:, 1, 7] = top.int(), -top.int()
+    x = torch.where(steps < 0, steps.abs() | -2 ** 31, steps).view(torch.float32)  # steps of 2^-149 are the bits
+    cache.append(batch, x, x)
+    k, v = cache.read(batch, n)
+    cache.status()
+    want = R.held(*R.quantise(x, 8), 8).float()
+    assert torch.equal(k, want) and torch.equal(v, want)
