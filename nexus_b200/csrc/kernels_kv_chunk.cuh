@@ -8,8 +8,8 @@
 // queries), the weights p sv rounded to f16 (hi + lo for f32).  ref is a whole
 // number chosen so that the largest p * max(sv, |zv|) of the row lies between
 // 2^(kUp-1) and f16's end; it moves only when a weight would pass that, and then
-// by an exact power of two (p alone is kept below 2^60 where values are zero, and
-// the values' scales are brought near one first, as there).
+// by an exact power of two (p alone is kept below 2^96 where values are zero, and
+// the values' scales are lifted first, as there).
 //
 // Bound: the tensor pipe (4 D flops a visible pair) and, next to it, the
 // shared-memory bandwidth that feeds it.  One CTA an SM, 256 rows (row r: token
@@ -62,7 +62,7 @@ static_assert(2 * kRegsSoftmax + kRegsProducer + kRegsIssue <= 4 * kRegsLaunch &
 constexpr int kBlk = 128 * 128;         // 128 rows x 64 f16, swizzled
 constexpr float kUp = 4.0f;             // a new reference puts the largest weight at 2^3 .. 2^4
 constexpr float kMaxWeight = 65504.0f;  // and it is moved when a weight would leave f16
-constexpr float kMaxProb = 60.0f;       // log2 of the largest p where values are zero
+constexpr float kMaxProb = kvf::kMaxProb;  // log2 of the largest p where values are zero
 constexpr int kScaleSlots = 4;
 constexpr int kFlush = kKvFlushTiles;
 
@@ -446,8 +446,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
                                (p.window == 0 || j0 > last - (int)p.window || j0 + kTok <= (int)p.sinks);
             unit = lds1(sl + Slot::UNIT);
             const float svmax = max4(lds4(sl + Slot::SMAX));
-            // largest sum of p over a thread's columns of a row: 2^80, and 2^100 / |zv|
-            const float plim = BV == 8 ? 1.2e24f : 1.2e30f / fmaxf(max4(lds4(sl + Slot::ZMAX)), 1e6f);
+            // largest sum of p over a thread's columns of a row: 2^99 (the eight of them at
+            // kMaxProb), and 2^100 / |zv|
+            const float plim = BV == 8 ? 6.4e29f : 1.27e30f / fmaxf(max4(lds4(sl + Slot::ZMAX)), 2.0f);
             const float fast_lim = fminf(plim, kMaxWeight / svmax);  // sums of p up to this keep every weight in f16
             const uint32_t slc = sl + 8 * c;  // this thread's columns: 8 k + 2 c and the next
 
@@ -510,13 +511,17 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
                         my[k] = fmaxf(my[k], __shfl_xor_sync(0xffffffffu, my[k], o));
                     }
                     const float next = fmaxf(ref[k], fmaxf(ceilf(my[k]) - kUp, ceilf(mx[k]) - kMaxProb));
-                    f[k] = next == ref[k] ? 1.0f : pow2_diff(ref[k], next);
+                    f[k] = 1.0f;
+                    if (next != ref[k]) {
+                        const kvf::Pow2 fl(ref[k], next);
+                        f[k] = pow2_diff(ref[k], next);
+                        l2[k] = mul2(mul2(l2[k], pk(fl.h, fl.h)), pk(fl.g, fl.g));
+                    }
                     ref[k] = next;
                     nref2[k] = next == -INFINITY ? pk(0.0f, 0.0f) : pk(-next, -next);
                     unset |= next == -INFINITY;
                     moved |= f[k] != 1.0f;
                     if constexpr (SPLIT) sum_f[k] *= f[k];
-                    l2[k] = mul2(l2[k], pk(f[k], f[k]));
                     z2[k] = mul2(z2[k], pk(f[k], f[k]));
                 }
                 if (!__any_sync(0xffffffffu, moved)) return;
@@ -730,10 +735,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
                     for (int u = 0; u < 4; u++) {
                         // positions of elements 0..7 within a unit of value codes
                         constexpr int i8[8] = {0, 1, 2, 3, 4, 5, 6, 7}, i4[8] = {0, 2, 4, 6, 1, 3, 5, 7};
-                        const float f = split_part ? unit : unit * inv;
+                        // (unit / l by itself may be below f32's normal numbers)
+                        const float f = split_part ? 1.0f : inv;
                         float v[8];
 #pragma unroll
-                        for (int e = 0; e < 8; e++) v[e] = (o[8 * u + (BV == 8 ? i8[e] : i4[e])] + z) * f;
+                        for (int e = 0; e < 8; e++) v[e] = (o[8 * u + (BV == 8 ? i8[e] : i4[e])] + z) * f * unit;
                         const int ch = (d0 - p0 + 8 * u) * wide / 16;
                         if (SPLIT || split_part) {
                             sts4(row + ((ch ^ (lane & swz)) << 4), __float_as_uint(v[0]), __float_as_uint(v[1]),
@@ -899,8 +905,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
                     }
                     mag = warp_max(mag);
                     if (mag > 0.0f) {
-                        lift = __int_as_float((127 + kvf::near_one(mag)) << 23);
-                        unit = __int_as_float((127 - kvf::near_one(mag)) << 23);
+                        lift = __int_as_float((127 + kvf::value_lift(mag)) << 23);
+                        unit = __int_as_float((127 - kvf::value_lift(mag)) << 23);
                     }
                 }
 #pragma unroll

@@ -15,9 +15,11 @@
 // it is set and is set anew when that passes 2^15: rescaling is by exact powers
 // of two, and whatever the scale of the values the weights stay in f16's range
 // with their 11 bits down to 2^-23 of the largest.  Where the values are zero
-// only p bounds m (2^60 at most); so that p never has to make up for values of
-// an extreme magnitude, scales and zeros are first brought near one by a power
-// of two taken from the first tile whose values are not all zero.
+// only p bounds m (2^96 at most, and 2^31 of those stay in f32).  p makes up for
+// the magnitude of the values, which later tiles may change at will: for scales
+// and zeros from 2^-86 to beyond 2^100.  Where the first tile that is not all
+// zero has nothing above 2^-80, or something above 2^40, scales and zeros are
+// multiplied by a power of two first (value_lift).
 //
 // Bound: HBM, the visible codes and scales once (264 bytes a token and head at
 // D = 128 and 8 bits, 144 at 4).  Layout:
@@ -51,7 +53,7 @@ constexpr int kStages = 3;
 // slots used)
 constexpr float kUp = 10.0f;         // log2 of the largest weight under a new reference
 constexpr float kLimit = 32768.0f;   // largest weight any reference stays for
-constexpr float kMaxProb = 60.0f;    // log2 of the largest p
+constexpr float kMaxProb = 96.0f;    // log2 of the largest p
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -87,12 +89,26 @@ __device__ __forceinline__ float lg2(float x) {
     asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// 2^(a - b) exactly, for whole a and b, either possibly -inf (0 then); the
-// exponent is kept within f32's normal range
+// 2^(a - b) exactly, for whole a <= b, either possibly -inf (0 then); 0 below f32's
+// normal range.  For sums of weights, which a factor below that leaves nothing of
+// (2^15 times their number, against 2^9 at least for the key that moved the reference).
 __device__ __forceinline__ float pow2_diff(float a, float b) {
-    if (a == -INFINITY || b == -INFINITY) return 0.0f;
-    return __int_as_float((127 + (int)fminf(126.0f, fmaxf(-126.0f, a - b))) << 23);
+    const float d = a - b;
+    return d >= -126.0f ? __int_as_float((127 + (int)d) << 23) : 0.0f;
 }
+// The same for sums of p: those of keys whose values are small are as large against the
+// others' as their scores say, however far the references are apart (p lies between 2^-126
+// and 2^96): a factor in two halves, each a normal number.
+struct Pow2 {
+    float h, g;
+    __device__ __forceinline__ Pow2(float a, float b) {
+        const float d = a - b;
+        const int e = d >= -252.0f ? (int)d : -252;
+        h = __int_as_float((127 + e / 2) << 23);
+        g = d >= -252.0f ? __int_as_float((127 + e - e / 2) << 23) : 0.0f;
+    }
+    __device__ __forceinline__ float times(float v) const { return v * h * g; }
+};
 
 // O += V^T P^T of one tile.  The tensor cores round each sum toward zero, an error
 // that grows with the number of tiles summed in place (2.2e-5 of the output after
@@ -146,9 +162,12 @@ __device__ __forceinline__ void lds_words(const uint8_t *p, uint32_t (&w)[N], in
     }
 }
 
-// Exponent that brings a positive magnitude near one, or within p's 2^60 of it.
-__device__ __forceinline__ int near_one(float mag) {
-    return min(60, max(-60, 127 - (int)((__float_as_uint(mag) >> 23) & 0xffu)));
+// log2 of what scales and zeros are multiplied by when the largest of the first tile that is
+// not all zero is `mag`.  Down, so that p stays clear of f32's lower end (2^-36 and more for a
+// value near 2^40); up by no more than 2^24, so that later values up to 2^104 stay in f32.
+__device__ __forceinline__ int value_lift(float mag) {
+    const int e = (int)((__float_as_uint(mag) >> 23) & 0xffu) - 127;
+    return e > 40 ? 40 - e : e < -80 ? 24 : 0;
 }
 // ---- distributed shared memory of a cluster ----
 __device__ __forceinline__ void cluster_sync() {
@@ -168,8 +187,10 @@ __device__ __forceinline__ float cluster_ld(uint32_t addr) {
 __device__ __forceinline__ void join(float &m, float &l, float (&v)[8], float m1, float l1, const float (&v1)[8]) {
     const float top = fmaxf(m, m1);
     const float f = m == top ? 1.0f : pow2_diff(m, top), f1 = m1 == top ? 1.0f : pow2_diff(m1, top);
+    const float low = fminf(m, m1);
+    if (low < top - 126.0f && low != -INFINITY) l = Pow2(m, top).times(l) + Pow2(m1, top).times(l1);
+    else l = fmaf(l1, f1, l * f);
     m = top;
-    l = fmaf(l1, f1, l * f);
 #pragma unroll
     for (int j = 0; j < 8; j++) v[j] = fmaf(v1[j], f1, v[j] * f);
 }
@@ -435,8 +456,8 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? (SPLIT ? 3 : 4) : 2) k_
                         mag = fmaxf(mag, fmaxf(sv[t], fabsf(zv[t])));
                 mag = warp_max(mag);
                 if (mag > 0.0f) {
-                    lift = __int_as_float((127 + near_one(mag)) << 23);
-                    unit = __int_as_float((127 - near_one(mag)) << 23);
+                    lift = __int_as_float((127 + value_lift(mag)) << 23);
+                    unit = __int_as_float((127 - value_lift(mag)) << 23);
                 }
             }
 #pragma unroll
@@ -482,8 +503,8 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? (SPLIT ? 3 : 4) : 2) k_
                         ww[nr][t] = mul2(pp[nr][t], pk(v0, v1));
                         float w0, w1;
                         upk(ww[nr][t], w0, w1);
-                        // a weight above 2^15, or p above 2^60
-                        top = fmaxf(fmaxf(top, fmaxf(w0, w1)), fmaxf(p0, p1) * 2.8421709e-14f);
+                        // a weight above 2^15, or p above 2^96
+                        top = fmaxf(fmaxf(top, fmaxf(w0, w1)), fmaxf(p0, p1) * 4.1359031e-25f);
                     }
                 if (!last_try && __any_sync(0xffffffffu, top > kLimit)) return false;
 #pragma unroll
@@ -517,7 +538,7 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? (SPLIT ? 3 : 4) : 2) k_
                     float x[2][2];
 #pragma unroll
                     for (int t = 0; t < 2; t++) upk(mul2(score(nr, t), x_scale[nr]), x[t][0], x[t][1]);
-                    float cm[2];
+                    float cm[2], ch[2], cg[2];
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
                         float mx = -INFINITY, my = -INFINITY;
@@ -533,12 +554,18 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? (SPLIT ? 3 : 4) : 2) k_
                             my = fmaxf(my, __shfl_xor_sync(0xffffffffu, my, w));
                         }
                         const float m1 = fmaxf(m[nr][e], fmaxf(ceilf(mx) - kMaxProb, ceilf(my) - kUp));
-                        cm[e] = m1 == m[nr][e] ? 1.0f : pow2_diff(m[nr][e], m1);
+                        cm[e] = ch[e] = cg[e] = 1.0f;
+                        if (m1 != m[nr][e]) {
+                            const Pow2 f(m[nr][e], m1);
+                            cm[e] = pow2_diff(m[nr][e], m1);
+                            ch[e] = f.h;
+                            cg[e] = f.g;
+                        }
                         m[nr][e] = m1;
                         unset |= m1 == -INFINITY;
                     }
                     nm[nr] = pk(m[nr][0] == -INFINITY ? 0.0f : -m[nr][0], m[nr][1] == -INFINITY ? 0.0f : -m[nr][1]);
-                    l[nr] = mul2(l[nr], pk(cm[0], cm[1]));
+                    l[nr] = mul2(mul2(l[nr], pk(ch[0], ch[1])), pk(cg[0], cg[1]));
                     z[nr] = mul2(z[nr], pk(cm[0], cm[1]));
 #pragma unroll
                     for (int j = 0; j < MT; j++)

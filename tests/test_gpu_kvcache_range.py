@@ -100,3 +100,25 @@ def test_append_subnormal_groups(backend, nb):
     cache.status()
     want = R.held(*R.quantise(x, 8), 8).float()
     assert torch.equal(k, want) and torch.equal(v, want)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("bits_v", [8, 4])
+@pytest.mark.parametrize("new", [1, 4, 80, 300])
+@pytest.mark.parametrize("first,then", [(1e-30, 1e25), (1e25, 1e-30), (1e-30, 1.0), (1.0, 1e30), (0.0, 1e-30)])
+def test_values_far_apart_in_one_sequence(backend, nb, first, then, new, bits_v, dtype):
+    """The magnitude of the first tiles' values says nothing about the later ones'."""
+    lens = [(new, new + 600), (new, new + 700)]
+    batch, pages, rows = make_batch(nb, lens, 16)
+    cache = nb.PagedKvCache.empty(backend, pages, 2, 64, 16, (8, bits_v))
+    fill_random(cache, 73)
+    for b in range(2):
+        ids = batch.page_table[b].long()
+        cache.v_scales[ids[:20]] *= first
+        cache.v_scales[ids[20:-(-lens[b][1] // 16)]] *= then
+    q = torch.randn((rows, 8, 64), generator=gen(74), device=DEV).to(DTYPES[dtype])
+    out = cache.attention(batch, q)
+    cache.status()
+    parts = R.attention(q, cache, lens, batch.page_table)
+    tol = R.tolerance(*parts, q.dtype) - 1e-30 + 2.0 ** -149  # relative to the values, however small they are
+    assert bool(((out.double() - parts[0]).abs() <= tol).all())
