@@ -7,9 +7,9 @@
 // kc, vc integer codes around zero (exact in f16), q as f16 (hi + lo for f32
 // queries), the weights p sv rounded to f16 (hi + lo for f32).  ref is a whole
 // number chosen so that the largest p * max(sv, |zv|) of the row lies between
-// 2^(kUp-1) and f16's end; it moves only when a weight would pass that, and then
-// by an exact power of two (p alone is kept below 2^96 where values are zero, and
-// the values' scales are lifted first, as there).
+// 2^(kUp-1) (kUpSplit for f32 queries) and f16's end; it moves only when a weight
+// would pass that, and then by an exact power of two (p alone is kept below 2^96
+// where values are zero, and the values' scales are lifted first, as there).
 //
 // Bound: the tensor pipe (4 D flops a visible pair) and, next to it, the
 // shared-memory bandwidth that feeds it.  One CTA an SM, 256 rows (row r: token
@@ -60,7 +60,13 @@ constexpr int kThreads = 16 * 32;
 constexpr int kRegsLaunch = 128, kRegsSoftmax = 160, kRegsProducer = 120, kRegsIssue = 72;
 static_assert(2 * kRegsSoftmax + kRegsProducer + kRegsIssue <= 4 * kRegsLaunch && kThreads * kRegsLaunch <= 65536, "more registers than the block has");
 constexpr int kBlk = 128 * 128;         // 128 rows x 64 f16, swizzled
-constexpr float kUp = 4.0f;             // a new reference puts the largest weight at 2^3 .. 2^4
+// A new reference puts the largest weight at 2^(kUp-1) .. 2^kUp, as low as 16 bits of output
+// allow: the lower, the less often it moves.  f16 ends at 2^-25, so that a weight is off
+// by up to 2^-28 of the largest besides its own rounding, which 2^17 keys that all lie there
+// make half a step of an f16 output.  f32 queries: 2^-35, 4e-6 of the leading value
+// for 2^17 such keys (a 2048-token prompt took 136 us at 4, 140 at 10, 142 at 11, 152 at 12,
+// where the sums of weights near the largest already reach f16's end).
+constexpr float kUp = 4.0f, kUpSplit = 11.0f;
 constexpr float kMaxWeight = 65504.0f;  // and it is moved when a weight would leave f16
 constexpr float kMaxProb = kvf::kMaxProb;  // log2 of the largest p where values are zero
 constexpr int kScaleSlots = 4;
@@ -446,8 +452,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
                                (p.window == 0 || j0 > last - (int)p.window || j0 + kTok <= (int)p.sinks);
             unit = lds1(sl + Slot::UNIT);
             const float svmax = max4(lds4(sl + Slot::SMAX));
-            // largest sum of p over a thread's columns of a row: 2^99 (the eight of them at
-            // kMaxProb), and 2^100 / |zv|
+            // largest sum of p over four columns of a row: 2^99 (each of them at kMaxProb,
+            // twice over), and 2^100 / |zv|
             const float plim = BV == 8 ? 6.4e29f : 1.27e30f / fmaxf(max4(lds4(sl + Slot::ZMAX)), 2.0f);
             const float fast_lim = fminf(plim, kMaxWeight / svmax);  // sums of p up to this keep every weight in f16
             const uint32_t slc = sl + 8 * c;  // this thread's columns: 8 k + 2 c and the next
@@ -510,7 +516,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
                         mx[k] = fmaxf(mx[k], __shfl_xor_sync(0xffffffffu, mx[k], o));
                         my[k] = fmaxf(my[k], __shfl_xor_sync(0xffffffffu, my[k], o));
                     }
-                    const float next = fmaxf(ref[k], fmaxf(ceilf(my[k]) - kUp, ceilf(mx[k]) - kMaxProb));
+                    const float next = fmaxf(ref[k], fmaxf(ceilf(my[k]) - (SPLIT ? kUpSplit : kUp), ceilf(mx[k]) - kMaxProb));
                     f[k] = 1.0f;
                     if (next != ref[k]) {
                         const kvf::Pow2 fl(ref[k], next);
@@ -555,7 +561,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
                 }
             };
             // The weights of columns 32 q .. + 31 against the references, and their sums.
-            // Returns the largest of the sums of p.
+            // Returns the largest of the sums of p (of four columns each).
             auto weigh = [&](auto masked, int q, const uint32_t(&cur)[2][16], uint32_t(&ph)[2][8], uint32_t(&pl)[2][8],
                              f2(&l_c)[4], f2(&z_c)[4]) -> float {
                 constexpr bool MASK = decltype(masked)::value;
@@ -596,7 +602,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
                 for (int k = 0; k < 4; k++) {
                     float a, b;
                     upk(l_c[k], a, b);
-                    sum[k] = a + b;
+                    sum[k] = fmaxf(a, b);
                 }
                 return fmaxf(fmaxf(sum[0], sum[1]), fmaxf(sum[2], sum[3]));
             };
@@ -645,7 +651,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
                 keep(on, q, ph, pl, l_c, z_c);
                 return on;
             };
-            // The old references are tried first; a weight is at most the sum of p times the
+            // The old references are tried first; a weight is at most a sum of p times the
             // largest scale, and from the first quarter where that says nothing on, the
             // second loop takes over with new ones.
             auto tile = [&](auto masked) {

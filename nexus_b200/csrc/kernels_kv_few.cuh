@@ -54,6 +54,10 @@ constexpr int kStages = 3;
 constexpr float kUp = 10.0f;         // log2 of the largest weight under a new reference
 constexpr float kLimit = 32768.0f;   // largest weight any reference stays for
 constexpr float kMaxProb = 96.0f;    // log2 of the largest p
+// f32 queries: what the second f16 of a weight is multiplied by (at most half a step of the
+// first, 2^3 for one of 2^15, so that it stays in f16).  A weight is then off by 2^-36 at
+// most where it is small, 2^-45 of the largest (by itself f16 ends at 2^-25).
+constexpr float kLoUp = 2048.0f;
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -113,6 +117,7 @@ struct Pow2 {
 // O += V^T P^T of one tile.  The tensor cores round each sum toward zero, an error
 // that grows with the number of tiles summed in place (2.2e-5 of the output after
 // 40000 tokens); for f32 queries a tile is summed alone and added correctly rounded.
+// Their weights' second halves come times 2^11 (kLoUp).
 template <int NS>
 __device__ __forceinline__ void add_tile(float (&o)[4], const uint32_t (&a)[4], const uint32_t (&p)[NS][2]) {
     if constexpr (NS == 1) {
@@ -120,6 +125,8 @@ __device__ __forceinline__ void add_tile(float (&o)[4], const uint32_t (&a)[4], 
     } else {
         float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         mma16816(t, a, p[1]);
+#pragma unroll
+        for (int i = 0; i < 4; i++) t[i] *= 1.0f / kLoUp;
         mma16816(t, a, p[0]);
 #pragma unroll
         for (int i = 0; i < 4; i++) o[i] += t[i];
@@ -524,7 +531,7 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? (SPLIT ? 3 : 4) : 2) k_
                         pf[nr][0][t] = transpose8x8(hi);
                         if constexpr (SPLIT) {
                             const float2 back = f16x2_back(hi);
-                            pf[nr][NS - 1][t] = transpose8x8(f16x2(w0 - back.x, w1 - back.y));
+                            pf[nr][NS - 1][t] = transpose8x8(f16x2((w0 - back.x) * kLoUp, (w1 - back.y) * kLoUp));
                         }
                     }
                 }

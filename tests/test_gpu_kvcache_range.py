@@ -1,4 +1,6 @@
 """Quantised paged KV cache on the GPU at the ends of its range: magnitudes, small weights, bad pages, padding."""
+import math
+
 import pytest
 import torch
 
@@ -122,3 +124,32 @@ def test_values_far_apart_in_one_sequence(backend, nb, first, then, new, bits_v,
     parts = R.attention(q, cache, lens, batch.page_table)
     tol = R.tolerance(*parts, q.dtype) - 1e-30 + 2.0 ** -149  # relative to the values, however small they are
     assert bool(((out.double() - parts[0]).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("kv", [20000, 100000])
+@pytest.mark.parametrize("new", [1, 60])
+def test_f32_keeps_many_small_weights(backend, nb, new, kv):
+    """Every sixteenth key leads by 21 nats, so that each part of the context has such keys: the others are
+    below what one f16 holds beside them.  In half of the dimensions the leading values are zero, so that
+    the small ones are all there is.
+
+    Two f16 of a weight lose at most 2^-35 of the leading one for each key: e^21 2^-35 of the small ones'
+    sum.  Besides that: scores and exp2 to 2^-18 of 21 nats (1e-4 of the small ones' sum), 2e-6 of the
+    whole as over other long contexts."""
+    batch, pages, rows = make_batch(nb, [(new, kv)], 64)
+    cache = nb.PagedKvCache.empty(backend, pages, 1, 64, 64, (8, 8))
+    g = gen(75)
+    cache.k_scales.fill_(0.01)
+    cache.v_scales.fill_(0.02)
+    cache.k_codes.copy_(torch.randint(126, 131, cache.k_codes.shape, generator=g, device=DEV, dtype=torch.uint8))
+    cache.v_codes.copy_(torch.randint(192, 256, cache.v_codes.shape, generator=g, device=DEV, dtype=torch.uint8))
+    q = torch.ones((rows, 4, 64), device=DEV) + 0.01 * torch.randn((rows, 4, 64), generator=g, device=DEV)
+    cache.k_codes[:, 0, ::16] = 128 + 100              # a score of 64 * 1.0 * scale
+    cache.v_codes[:, 0, ::16, :32] = 128               # zero
+    out = cache.attention(batch, q, scale=21.0 / 64)
+    cache.status()
+    ref = R.attention(q, cache, [(new, kv)], batch.page_table, scale=21.0 / 64)[0]
+    small = float((out[..., :32].double() - ref[..., :32]).norm() / ref[..., :32].norm())
+    whole = float((out.double() - ref).norm() / ref.norm())
+    assert whole < 2e-6, whole
+    assert small < 1e-4 + math.exp(21) * 2.0 ** -35, small
