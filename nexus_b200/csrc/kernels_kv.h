@@ -40,7 +40,14 @@ struct KvAttnParams {
     KvRows q, out;
     int group;
     uint32_t group_magic;      // ceil(2^32 / group), 0 for a group of one (kv_div)
-    float scale_log2;          // score scale * log2(e)
+    // score scale * log2(e) = key_scale 2^scale_exp, key_scale in [1, 2): the first goes on
+    // the keys' scales and zeros, so that what a row's scores are multiplied by is a power
+    // of two and x = score 2^n exact.  Then x - m is rounded once from the x that the
+    // reference m was taken from, and however many nats a step of f32 is at x, the largest
+    // key of a row has a weight near one (with the whole factor here, scores beyond 2^31
+    // left weights of 0 and infinity).
+    float key_scale;
+    int scale_exp;
     uint32_t window, sinks;
     unsigned *fault;
     // split over the context

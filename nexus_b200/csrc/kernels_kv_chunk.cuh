@@ -74,7 +74,7 @@ constexpr int kFlush = kKvFlushTiles;
 
 // What the softmax needs of a key tile, by token; byte offsets in shared memory.
 struct Slot {
-    static constexpr int SK = 0, ZK = 512, SV = 1024, ZV = 1536;
+    static constexpr int SK = 0, ZK = 512, SV = 1024, ZV = 1536;  // (the keys' times key_scale)
     static constexpr int LV = 2048;            // log2 max(sv, |zv|)
     static constexpr int SMAX = 2560, ZMAX = 2576;  // largest sv, |zv| of each quarter of the tokens
     static constexpr int UNIT = 2592;          // what sv and zv were divided by
@@ -340,7 +340,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
                 for (int i = 0; i < 8; i++) amax = fmaxf(amax, fabsf(q[i]));
 #pragma unroll
                 for (int o = LPR / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-                const float sc = row_scale(amax);
+                const int e_row = row_exp(amax);
+                const float sc = pow2i(7 - e_row);
                 // elements in the order the codes of a word unpack to
                 constexpr int o8[8] = {0, 1, 2, 3, 4, 5, 6, 7}, o4[8] = {0, 4, 1, 5, 2, 6, 3, 7};
                 uint32_t hi[4];
@@ -364,7 +365,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
                 sts4(dst, hi[0], hi[1], hi[2], hi[3]);
                 if constexpr (SPLIT) sts4(dst + S::DB * kBlk, lo[0], lo[1], lo[2], lo[3]);
                 if (cl == 0) {
-                    row_x[sub * 128 + rr] = p.scale_log2 / sc;
+                    row_x[sub * 128 + rr] = pow2i(p.scale_exp + e_row - 7);
                     row_sum[sub * 128 + rr] = sum;
                 }
             }
@@ -925,10 +926,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
                         rs[t][0] = kv_nan();
                         sv = zv = 0.0f;
                     }
-                    sts1(at + Slot::SK, rs[t][0]);
+                    sts1(at + Slot::SK, rs[t][0] * p.key_scale);
                     sts1(at + Slot::SV, sv);
                     sts1(at + Slot::LV, lg2(fmaxf(sv, fabsf(zv))));
-                    if constexpr (BK == 4) sts1(at + Slot::ZK, rs[t][1]);
+                    if constexpr (BK == 4) sts1(at + Slot::ZK, rs[t][1] * p.key_scale);
                     if constexpr (BV == 4) sts1(at + Slot::ZV, zv);
                     const float sm = warp_max(sv), zm = BV == 4 ? warp_max(fabsf(zv)) : 0.0f;
                     if (lane == 0) {

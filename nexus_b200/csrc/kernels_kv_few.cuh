@@ -296,6 +296,8 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? (SPLIT ? 3 : 4) : 2) k_
     // products cancel against zero - mid * scale, which costs f32 a few units in the
     // last place of the score (too many for f32 queries, whose codes are centred).
     constexpr bool RAW = !SPLIT;
+    constexpr float kRawUp = 16777216.0f;
+    const float key_factor = p.key_scale * (RAW ? kRawUp : 1.0f);
     uint32_t qf[NR][NS][KSTEPS][2];
     f2 x_scale[NR], x_sum[NR];  // of this thread's columns, rows 2c and 2c + 1
     int x_pos[NR][2];
@@ -323,7 +325,8 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? (SPLIT ? 3 : 4) : 2) k_
         }
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-        const float sc = row_scale(amax);
+        const int e_row = row_exp(amax);
+        const float sc = pow2i(7 - e_row);
         float sum = 0.0f;
 #pragma unroll
         for (int u = 0; u < UNITS; u++) {
@@ -349,9 +352,7 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? (SPLIT ? 3 : 4) : 2) k_
         }
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        // (the sum in the units of the raw products)
-        const float xs = p.scale_log2 / sc * (RAW ? 16777216.0f : 1.0f);
-        if constexpr (RAW) sum *= 1.0f / 16777216.0f;
+        const float xs = pow2i(p.scale_exp + e_row - 7);
         const int pos = used ? pos0 + (int)tok : -1;
         float xe[2], se[2];
 #pragma unroll
@@ -453,7 +454,9 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? (SPLIT ? 3 : 4) : 2) k_
                 zk[t] = BK == 8 ? 0.0f : kscale[2 * i + 1];
                 sv[t] = BV == 8 ? vscale[i] : vscale[2 * i];
                 zv[t] = BV == 8 ? 0.0f : vscale[2 * i + 1];
-                if constexpr (RAW) zk[t] = fmaf(BK == 8 ? -128.0f : -8.0f, sk[t], zk[t]);
+                sk[t] *= key_factor;
+                if constexpr (BK == 4) zk[t] *= p.key_scale;
+                if constexpr (RAW) zk[t] = fmaf((BK == 8 ? -128.0f : -8.0f) / kRawUp, sk[t], zk[t]);
             }
             if (lift == 0.0f) {
                 float mag = 0.0f;

@@ -160,13 +160,17 @@ __device__ __forceinline__ float max4(float4 v) { return fmaxf(fmaxf(v.x, v.y), 
 // the first n of 32 bits, any n
 __device__ __forceinline__ uint32_t first_bits(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
 
-// The power of two that brings a row whose largest magnitude is `amax` to
+// 2^e: the largest power of f32 above its range, 0 below it.
+__device__ __forceinline__ float pow2i(int e) {
+    return __int_as_float(e >= -126 ? (127 + min(e, 127)) << 23 : e >= -149 ? 1 << (149 + e) : 0);
+}
+// The exponent of a row's largest magnitude.  The row times 2^(7 - row_exp) lies in
 // [2^7, 2^8): the queries then fit f16 with 22 significant bits in hi + lo,
-// whatever their type (exponents beyond +-100 are left where they are).
-__device__ __forceinline__ float row_scale(float amax) {
-    int e = (int)((__float_as_uint(amax) >> 23) & 0xffu) - 127;
-    e = min(100, max(-100, e));
-    return __int_as_float((127 + 7 - e) << 23);
+// whatever their type (exponents beyond +-100 are left where they are).  What the
+// scores are multiplied by, 2^(scale_exp + row_exp - 7), is held at 2^127: scores of
+// keys near one are then beyond 2^111.
+__device__ __forceinline__ int row_exp(float amax) {
+    return min(100, max(-100, (int)((__float_as_uint(amax) >> 23) & 0xffu) - 127));
 }
 
 __device__ __forceinline__ void kv_report(unsigned *fault, unsigned bits) {

@@ -302,7 +302,9 @@ extern "C" int nexus_cuda_kv_attention(nexus_cuda_backend *b, const nexus_kv_cac
     p.out = rows_view(out);
     p.group = (int)(q->heads / cache->kv_heads);
     p.group_magic = kv_div_magic((uint32_t)p.group);
-    p.scale_log2 = (scale != 0.0f ? scale : 1.0f / sqrtf((float)cache->head_dim)) * 1.4426950408889634f;
+    p.key_scale = 2.0f * frexpf((scale != 0.0f ? scale : 1.0f / sqrtf((float)cache->head_dim)) * 1.4426950408889634f,
+                                &p.scale_exp);
+    p.scale_exp--;
     p.window = window;
     p.sinks = sinks;
     p.fault = nexus_backend_kv_fault(b);

@@ -153,3 +153,37 @@ def test_f32_keeps_many_small_weights(backend, nb, new, kv):
     whole = float((out.double() - ref).norm() / ref.norm())
     assert whole < 2e-6, whole
     assert small < 1e-4 + math.exp(21) * 2.0 ** -35, small
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("bits", [(8, 8), (4, 4)])
+@pytest.mark.parametrize("new", [1, 4, 60])
+@pytest.mark.parametrize("scale,size", [(1e8, 1.0), (1e10, 1.0), (1e20, 1.0), (1e30, 1.0), (1e34, 1.0), (2e38, 2.0 ** -10)])
+def test_scores_beyond_the_steps_of_f32(backend, nb, scale, size, new, bits, dtype):
+    """Scores so large that a step of f32 is many nats: the key with the largest takes all, the output is
+    its value (an f16 weight, 2^-11, or two for f32 queries; the output's rounding)."""
+    lens = [(new, 700), (new, 90)]
+    batch, pages, rows = make_batch(nb, lens, 16)
+    cache = nb.PagedKvCache.empty(backend, pages, 2, 64, 16, bits)
+    fill_random(cache, 76)
+    g = gen(77)
+    sign = torch.where(torch.rand(64, generator=g, device=DEV) < 0.5, -1.0, 1.0)
+    if bits[0] == 4:
+        cache.k_scales[..., 1] = 0.0                    # (the zero alone would give every key a part of the score)
+    for b, at in ((0, 333), (1, 20)):
+        page, slot = int(batch.page_table[b, at // 16]), at % 16
+        cache.k_codes[page, :, slot] = (torch.where(sign > 0, 255, 1) if bits[0] == 8 else
+                                        torch.where(sign > 0, 15, 1)[0::2] | torch.where(sign > 0, 240, 16)[1::2]
+                                        ).to(torch.uint8)
+        cache.k_scales[page, :, slot, 0] *= 2.0
+    q = (size * sign * (0.5 + torch.rand((rows, 8, 64), generator=g, device=DEV))).to(DTYPES[dtype])
+    out = cache.attention(batch, q, scale=scale)
+    cache.status()
+    for b, at in ((0, 333), (1, 20)):
+        page, slot = int(batch.page_table[b, at // 16]), at % 16
+        v, z = R.side(cache.v_codes[page, :, slot], cache.v_scales[page, :, slot], bits[1])
+        want = (v + z).repeat_interleave(4, 0).expand(new, 8, 64)
+        part = (v.abs() + z.abs()).repeat_interleave(4, 0).expand(new, 8, 64)
+        w = 2.0 ** -21 if dtype == "f32" else 2.0 ** -11
+        tol = torch.finfo(DTYPES[dtype]).eps / 2 * want.abs() + (w + 2.0 ** -20) * part
+        assert bool(((out[b * new:(b + 1) * new].double() - want).abs() <= tol).all())
