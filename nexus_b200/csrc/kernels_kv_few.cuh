@@ -296,8 +296,11 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? (SPLIT ? 3 : 4) : 2) k_
     // products cancel against zero - mid * scale, which costs f32 a few units in the
     // last place of the score (too many for f32 queries, whose codes are centred).
     constexpr bool RAW = !SPLIT;
-    constexpr float kRawUp = 16777216.0f;
-    const float key_factor = p.key_scale * (RAW ? kRawUp : 1.0f);
+    // Of the 2^24, 2^5 go on the keys' scales and 2^19 on the row's factor: neither leaves f32
+    // before the scores of centred codes would (keys of 2^114, queries times scale of 2^122).
+    constexpr int kNorm = RAW ? 14 : 7;
+    constexpr float kRawUp = 16777216.0f, kKeyUp = RAW ? 32.0f : 1.0f;
+    const float key_factor = p.key_scale * kKeyUp;
     uint32_t qf[NR][NS][KSTEPS][2];
     f2 x_scale[NR], x_sum[NR];  // of this thread's columns, rows 2c and 2c + 1
     int x_pos[NR][2];
@@ -326,7 +329,7 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? (SPLIT ? 3 : 4) : 2) k_
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
         const int e_row = row_exp(amax);
-        const float sc = pow2i(7 - e_row);
+        const float sc = pow2i(kNorm - e_row);
         float sum = 0.0f;
 #pragma unroll
         for (int u = 0; u < UNITS; u++) {
@@ -352,7 +355,8 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? (SPLIT ? 3 : 4) : 2) k_
         }
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        const float xs = pow2i(p.scale_exp + e_row - 7);
+        if constexpr (RAW) sum *= kKeyUp / kRawUp;  // (the sum in the scores' units)
+        const float xs = pow2i(p.scale_exp + e_row - kNorm + (RAW ? 24 - 5 : 0));
         const int pos = used ? pos0 + (int)tok : -1;
         float xe[2], se[2];
 #pragma unroll
@@ -456,7 +460,7 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? (SPLIT ? 3 : 4) : 2) k_
                 zv[t] = BV == 8 ? 0.0f : vscale[2 * i + 1];
                 sk[t] *= key_factor;
                 if constexpr (BK == 4) zk[t] *= p.key_scale;
-                if constexpr (RAW) zk[t] = fmaf((BK == 8 ? -128.0f : -8.0f) / kRawUp, sk[t], zk[t]);
+                if constexpr (RAW) zk[t] = fmaf((BK == 8 ? -128.0f : -8.0f) / kKeyUp, sk[t], zk[t]);
             }
             if (lift == 0.0f) {
                 float mag = 0.0f;

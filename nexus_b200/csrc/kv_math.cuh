@@ -164,13 +164,14 @@ __device__ __forceinline__ uint32_t first_bits(int n) { return n <= 0 ? 0u : n >
 __device__ __forceinline__ float pow2i(int e) {
     return __int_as_float(e >= -126 ? (127 + min(e, 127)) << 23 : e >= -149 ? 1 << (149 + e) : 0);
 }
-// The exponent of a row's largest magnitude.  The row times 2^(7 - row_exp) lies in
-// [2^7, 2^8): the queries then fit f16 with 22 significant bits in hi + lo,
-// whatever their type (exponents beyond +-100 are left where they are).  What the
-// scores are multiplied by, 2^(scale_exp + row_exp - 7), is held at 2^127: scores of
-// keys near one are then beyond 2^111.
+// The exponent of a row's largest magnitude, by which a row is brought to one magnitude
+// whatever its type: to [2^7, 2^8), where queries have 22 significant bits in f16 hi + lo,
+// or to [2^14, 2^15), where codes are met as they stand, 2^-24 each (rows below 2^-112
+// stay smaller than that, and their scores with any finite key are below 2^26).  What the
+// scores are multiplied by, 2^(scale_exp + row_exp) or so, is held at 2^127: scores of keys
+// near one are then beyond 2^111.
 __device__ __forceinline__ int row_exp(float amax) {
-    return min(100, max(-100, (int)((__float_as_uint(amax) >> 23) & 0xffu) - 127));
+    return min(127, max(-112, (int)((__float_as_uint(amax) >> 23) & 0xffu) - 127));
 }
 
 __device__ __forceinline__ void kv_report(unsigned *fault, unsigned bits) {

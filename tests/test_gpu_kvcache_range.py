@@ -187,3 +187,25 @@ def test_scores_beyond_the_steps_of_f32(backend, nb, scale, size, new, bits, dty
         w = 2.0 ** -21 if dtype == "f32" else 2.0 ** -11
         tol = torch.finfo(DTYPES[dtype]).eps / 2 * want.abs() + (w + 2.0 ** -20) * part
         assert bool(((out[b * new:(b + 1) * new].double() - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("bits_k", [8, 4])
+@pytest.mark.parametrize("new", [1, 4, 60])
+@pytest.mark.parametrize("power", [-110, -104, 109, 115, 120])
+def test_queries_of_any_magnitude(backend, nb, power, new, bits_k, dtype):
+    """Queries times 2^n against keys times 2^-n: the same scores to the last bit, the same output."""
+    lens = [(new, 300), (new, 61)]
+    batch, pages, rows = make_batch(nb, lens, 16)
+    cache = nb.PagedKvCache.empty(backend, pages, 2, 64, 16, (bits_k, 8))
+    fill_random(cache, 78)
+    if bits_k == 4:  # (nor of a zero)
+        zero = cache.k_scales[..., 1]
+        cache.k_scales[..., 1] = torch.where(zero < 0, -1.0, 1.0) * zero.abs().clamp(min=2.0 ** -4)
+    q = torch.randn((rows, 8, 64), generator=gen(79), device=DEV).to(DTYPES[dtype])
+    q = torch.where(q < 0, -1.0, 1.0).to(q.dtype) * q.abs().clamp(min=2.0 ** -4)  # no bit of it falls below f32's last
+    want = check_attention(cache, batch, lens, q)
+    cache.k_scales.mul_(2.0 ** -power)
+    got = cache.attention(batch, q * 2.0 ** power)
+    cache.status()
+    assert torch.equal(got.double(), want)
