@@ -552,6 +552,7 @@ int nexus_cuda_kv_attention_workspace(const nexus_kv_cache *cache, const nexus_k
 /* Waits for the stream (NULL with flags 0: the backend's) and reports, then
  * clears, what this backend's KV calls found wrong on the device:
  * NEXUS_E_INVALID with a message, NEXUS_E_TIMEOUT for a wait that gave up.
+ * Each fault is reported to one of the callers that ask at the same time.
  * Not for use during stream capture. */
 int nexus_cuda_kv_status(nexus_cuda_backend *b, void *stream, uint32_t flags);
 

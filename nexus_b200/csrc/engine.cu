@@ -49,8 +49,9 @@ struct nexus_cuda_backend {
     // set by a kernel whose bounded wait gave up (op-level calls)
     int *dev_err = nullptr;
     // what the paged KV cache calls found wrong on the device (kvcache.cu):
-    // [0] KvFault bits, [1] the bits nexus_cuda_kv_status takes
+    // [0] KvFault bits, [1] the bits nexus_cuda_kv_status takes (under kv_mu)
     unsigned *kv_fault = nullptr;
+    std::mutex kv_mu;
     // tensor parallelism (nexus_cuda_tp_init)
     int tp_rank = 0, tp_world = 1;
     ncclComm_t comm = nullptr;
@@ -315,6 +316,8 @@ int nexus_backend_stream_device(nexus_cuda_backend *b, cudaStream_t *stream, int
 }
 
 unsigned *nexus_backend_kv_fault(nexus_cuda_backend *b) { return b->kv_fault; }
+
+std::mutex &nexus_backend_kv_mutex(nexus_cuda_backend *b) { return b->kv_mu; }
 
 int nexus_backend_fail(nexus_cuda_backend *b, int code, const char *msg) {
     try {

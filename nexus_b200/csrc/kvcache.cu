@@ -8,6 +8,8 @@
 #include <cuda_runtime.h>
 #include <math.h>
 
+#include <mutex>
+
 #include "../../include/nexus_cuda.h"
 #include "kernels_kv.h"
 
@@ -17,6 +19,7 @@ using namespace nx;
 extern int nexus_backend_stream_device(nexus_cuda_backend *b, cudaStream_t *stream, int *device);
 extern int nexus_backend_fail(nexus_cuda_backend *b, int code, const char *msg);
 extern unsigned *nexus_backend_kv_fault(nexus_cuda_backend *b);
+extern std::mutex &nexus_backend_kv_mutex(nexus_cuda_backend *b);
 
 namespace {
 
@@ -343,12 +346,16 @@ extern "C" int nexus_cuda_kv_status(nexus_cuda_backend *b, void *stream, uint32_
     if (r == cudaSuccess && cap != cudaStreamCaptureStatusNone)
         return nexus_backend_fail(b, NEXUS_E_INVALID, "kv status: the stream is being captured");
     unsigned *fault = nexus_backend_kv_fault(b), bits = 0;
+    // (the wait is outside the lock: callers on other streams need not share it)
+    if (r == cudaSuccess) r = cudaStreamSynchronize(st);
     if (r == cudaSuccess) {
+        // the word that the bits are taken to is the backend's: one caller at a time
+        std::lock_guard<std::mutex> lk(nexus_backend_kv_mutex(b));
         k_kv_take_fault<<<1, 1, 0, st>>>(fault);
         r = cudaGetLastError();
+        if (r == cudaSuccess) r = cudaMemcpyAsync(&bits, fault + 1, sizeof(bits), cudaMemcpyDeviceToHost, st);
+        if (r == cudaSuccess) r = cudaStreamSynchronize(st);
     }
-    if (r == cudaSuccess) r = cudaMemcpyAsync(&bits, fault + 1, sizeof(bits), cudaMemcpyDeviceToHost, st);
-    if (r == cudaSuccess) r = cudaStreamSynchronize(st);
     if (r != cudaSuccess) return cuda_fail(b, r);
     if (bits & KV_FAULT_WAIT)
         return nexus_backend_fail(b, NEXUS_E_TIMEOUT, "kv: a kernel's bounded wait gave up (asynchronous copy or MMA never completed)");

@@ -1,5 +1,6 @@
-"""Quantised paged KV cache on the GPU at the ends of its range: magnitudes, small weights, bad pages, padding."""
+"""Quantised paged KV cache on the GPU at the ends of its range: magnitudes, small weights, bad pages, padding, callers at once."""
 import math
+import threading
 
 import pytest
 import torch
@@ -209,3 +210,38 @@ def test_queries_of_any_magnitude(backend, nb, power, new, bits_k, dtype):
     got = cache.attention(batch, q * 2.0 ** power)
     cache.status()
     assert torch.equal(got.double(), want)
+
+
+def test_a_fault_is_reported_to_one_of_many_callers(backend, nb):
+    """status() from eight threads on streams of their own: each fault is reported once."""
+    batch, pages, rows = make_batch(nb, [(1, 40)], 16)
+    cache = nb.PagedKvCache.empty(backend, pages, 2, 64)
+    q = torch.zeros((1, 4, 64), device=DEV)
+    batch.page_table[0, 1] = pages
+    streams = [torch.cuda.Stream() for _ in range(8)]
+    start, end, told = threading.Barrier(9, timeout=60), threading.Barrier(9, timeout=60), []
+
+    def ask(stream):
+        with torch.cuda.stream(stream):
+            for _ in range(200):
+                start.wait()
+                try:
+                    cache.status()
+                except nb.NexusError as e:
+                    told.append(str(e))
+                end.wait()
+    threads = [threading.Thread(target=ask, args=(s,)) for s in streams]
+    for t in threads:
+        t.start()
+    counts = []
+    for _ in range(200):
+        cache.attention(batch, q)
+        torch.cuda.synchronize()
+        before = len(told)
+        start.wait()
+        end.wait()
+        counts.append(len(told) - before)
+    for t in threads:
+        t.join()
+    assert counts == [1] * 200
+    assert all("page" in m for m in told)
