@@ -128,7 +128,8 @@ int nexus_cuda_memory_info(nexus_cuda_backend *b, size_t *total, size_t *free_by
                            size_t *used);
 /* Backend::synchronize (src/backend/mod.rs:95) */
 int nexus_cuda_synchronize(nexus_cuda_backend *b);
-/* Last error message for this backend (thread-local when b is NULL). */
+/* Last error message for this backend (thread-local when b is NULL); the text
+ * is the calling thread's until it asks for this backend's again. */
 const char *nexus_cuda_last_error(const nexus_cuda_backend *b);
 
 /* ---- Tensor parallelism (one process per GPU) ----

@@ -12,6 +12,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <map>
 #include <memory>
 #include <mutex>
 #include <string>
@@ -155,8 +156,14 @@ static void backend_release(nexus_cuda_backend *b) {
     if (free_now) backend_free_now(b);
 }
 
+// Backends' messages: written by whichever thread's call fails, read by any.
+static std::mutex g_error_mu;
+
 static int set_err(nexus_cuda_backend *b, int code, const std::string &msg) {
-    if (b) b->last_error = msg;
+    if (b) {
+        std::lock_guard<std::mutex> lk(g_error_mu);
+        b->last_error = msg;
+    }
     g_tls_error = msg;
     return code;
 }
@@ -321,8 +328,6 @@ std::mutex &nexus_backend_kv_mutex(nexus_cuda_backend *b) { return b->kv_mu; }
 
 int nexus_backend_fail(nexus_cuda_backend *b, int code, const char *msg) {
     try {
-        static std::mutex mu;  // calls from several threads may fail at once
-        std::lock_guard<std::mutex> lk(mu);
         return set_err(b, code, msg);
     } catch (...) {  // no memory for the message: the status stands alone
         return code;
@@ -658,7 +663,17 @@ extern "C" int nexus_cuda_tp_init(nexus_cuda_backend *b, int rank, int world, co
 }
 
 extern "C" const char *nexus_cuda_last_error(const nexus_cuda_backend *b) {
-    return b ? b->last_error.c_str() : g_tls_error.c_str();
+    if (!b) return g_tls_error.c_str();
+    // the reader's own copy: another thread's call may fail while it is read
+    static thread_local std::map<const nexus_cuda_backend *, std::string> copies;
+    try {
+        std::string &copy = copies[b];
+        std::lock_guard<std::mutex> lk(g_error_mu);
+        copy = b->last_error;
+        return copy.c_str();
+    } catch (...) {
+        return "no memory for the message";
+    }
 }
 
 // ---------------------------------------------------------------------------

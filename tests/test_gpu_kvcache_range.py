@@ -245,3 +245,31 @@ def test_a_fault_is_reported_to_one_of_many_callers(backend, nb):
         t.join()
     assert counts == [1] * 200
     assert all("page" in m for m in told)
+
+
+def test_messages_of_calls_that_fail_at_once(backend, nb):
+    """Refused calls on four threads: every message read is one of theirs, whole."""
+    batch, pages, rows = make_batch(nb, [(1, 20)], 16)
+    cache = nb.PagedKvCache.empty(backend, pages, 2, 64)
+    three, one = torch.zeros((1, 3, 64), device=DEV), torch.zeros((1, 4, 64), device=DEV)
+    calls = (lambda: cache.attention(batch, three), lambda: cache.attention(batch, one, scale=3e38),
+             lambda: cache.append(batch, one, one), lambda: cache.attention(batch, one, out=one.expand(1, 4, 64)[:, :2]))
+    known, told, lock = set(), set(), threading.Lock()
+
+    def refused(call):
+        with pytest.raises(nb.NexusError) as e:
+            call()
+        return str(e.value)
+    for call in calls:
+        known.add(refused(call))
+
+    def repeat(call):
+        mine = {refused(call) for _ in range(2000)}
+        with lock:
+            told.update(mine)
+    threads = [threading.Thread(target=repeat, args=(c,)) for c in calls]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(known) == 4 and told <= known
