@@ -13,12 +13,12 @@ from .scheduler import ContinuousBatcher, KvPageAllocation, ScheduledDecode, Sch
 __all__ = ["_lib", "F32", "F16", "BF16", "Q4_0", "Q8_0", "Q2_K", "Q4_K", "FORMAT_IDS", "FORMAT_NAMES",
            "NexusError", "BackendCapabilities", "CudaBackend", "InferenceEngine", "MemoryInfo", "QWeight",
            "cuda_capabilities", "quantize_host", "tp_plan", "tp_unique_id", "write_synthetic_model", "CONFIGS",
-           "model_path", "Scheduler", "ScheduledDecode", "KvPageAllocation", "ContinuousBatcher", "ServeEvent",
-           "PagedKvCache", "KvBatch"]
+           "model_path", "Scheduler", "ScheduledDecode", "KvPageAllocation", "ContinuousBatcher", "ServeEvent"]
 
 
 def __getattr__(name):
     # the paged KV cache works on torch tensors; torch is imported when it is first used
+    # (and so these two are not in __all__: a star import works without torch)
     if name in ("PagedKvCache", "KvBatch"):
         from . import paged
         return getattr(paged, name)

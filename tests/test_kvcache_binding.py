@@ -1,6 +1,12 @@
 """The Python binding of the quantised paged KV cache without a GPU: what it hands to the C calls, and its refusals."""
+import subprocess
+import sys
+from pathlib import Path
+
 import pytest
 import torch
+
+ROOT = Path(__file__).resolve().parents[1]
 
 
 class OnGpu(torch.Tensor):
@@ -24,3 +30,25 @@ def test_a_slice_of_a_table_bounds_its_sequences(nb):
     assert batch._ref(0, 64)._obj.max_kv == 200  # pages of 64 tokens hold 256
     assert batch._ref(0, 16)._obj.max_kv == 64
     assert batch.max_kv == 200
+
+
+def test_the_package_needs_no_torch_until_the_cache_is_used():
+    """A star import without torch works; the names of the paged cache ask for it."""
+    code = """
+import sys
+sys.modules["torch"] = None   # import torch raises ImportError
+from nexus_b200 import *
+CudaBackend, Scheduler
+import nexus_b200
+try:
+    nexus_b200.PagedKvCache
+except ImportError:
+    print("asked")
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True)
+    assert r.returncode == 0 and r.stdout == "asked\n", r.stderr
+
+
+def test_the_paged_cache_is_a_name_of_the_package(nb):
+    from nexus_b200 import KvBatch, PagedKvCache
+    assert nb.KvBatch is KvBatch and nb.PagedKvCache is PagedKvCache
