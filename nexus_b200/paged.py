@@ -28,6 +28,7 @@ from . import _lib as L
 from .engine import CudaBackend
 
 _FORMATS = {torch.float32: L.F32, torch.float16: L.F16, torch.bfloat16: L.BF16}
+_KEPT = 64  # structs and sizes a batch keeps (a long-lived one may meet any number of streams)
 _raw_stream = torch._C._cuda_getCurrentRawStream  # torch.cuda.current_stream().cuda_stream without its object
 
 
@@ -43,7 +44,8 @@ def _on(t: torch.Tensor, device: torch.device, what: str) -> None:
 class KvBatch:
     """A ragged batch: sequence b brings rows q_start[b]..q_start[b + 1] of the
     row tensors, the last of its kv_len[b] tokens; token t lives in page
-    page_table[b, t // page_tokens].  int32 CUDA tensors (kept by reference);
+    page_table[b, t // page_tokens].  int32 CUDA tensors (kept by reference:
+    their contents may change between calls, not which tensors they are);
     max_q and max_kv bound the new tokens and the length of any sequence, as
     the columns of page_table (which may be a slice of a wider table) do."""
 
@@ -68,17 +70,41 @@ class KvBatch:
             raise _invalid("batch arrays are on different devices")
         if not (0 <= max_q < 1 << 31 and 0 <= max_kv < 1 << 31):
             raise _invalid("max_q and max_kv must be in [0, 2^31)")
-        self.q_start, self.kv_len, self.page_table = q_start, kv_len, page_table
-        self.max_q, self.max_kv = int(max_q), int(max_kv)
+        self._tensors = q_start, kv_len, page_table
+        self._bounds = int(max_q), int(max_kv)
         self._args = (page_table.stride(0) if n > 1 else page_table.shape[1], q_start.data_ptr(), kv_len.data_ptr(),
                       page_table.data_ptr())
         self._index = kv_len.get_device()
         self._structs = {}     # by stream and page size: filled once, never changed
         self._workspaces = {}  # bytes by what they depend on
 
+    # What the calls are handed was taken from these once: contents may change, the
+    # tensors and the bounds are another batch's.
+    @property
+    def q_start(self) -> torch.Tensor:
+        return self._tensors[0]
+
+    @property
+    def kv_len(self) -> torch.Tensor:
+        return self._tensors[1]
+
+    @property
+    def page_table(self) -> torch.Tensor:
+        return self._tensors[2]
+
+    @property
+    def max_q(self) -> int:
+        return self._bounds[0]
+
+    @property
+    def max_kv(self) -> int:
+        return self._bounds[1]
+
     def _ref(self, stream: int, page_tokens: int):
         r = self._structs.get((stream, page_tokens))
         if r is None:
+            if len(self._structs) >= _KEPT:
+                self._structs.clear()
             # the rows of a table that is a slice of a wider one are further apart than they
             # have entries: a sequence ends with its entries, not with the row's pitch
             max_kv = min(self.max_kv, self.page_table.shape[1] * page_tokens)
@@ -200,6 +226,8 @@ class PagedKvCache:
         if need is None:
             size = C.c_size_t()
             L.check(self._lib.nexus_cuda_kv_attention_workspace(self._ref, bt, qr, window, sinks, C.byref(size)))
+            if len(batch._workspaces) >= _KEPT:
+                batch._workspaces.clear()
             need = batch._workspaces[key] = size.value
         # (held until the launch; reused by the allocator in stream order after it)
         ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None

@@ -52,3 +52,22 @@ except ImportError:
 def test_the_paged_cache_is_a_name_of_the_package(nb):
     from nexus_b200 import KvBatch, PagedKvCache
     assert nb.KvBatch is KvBatch and nb.PagedKvCache is PagedKvCache
+
+
+def test_a_batch_is_of_its_tensors_and_bounds_for_good(nb):
+    """The struct handed to the calls holds their addresses: another tensor is another batch."""
+    batch = nb.KvBatch(i32(4), i32(3), i32(3, 8), 2, 100)
+    kept = batch.kv_len
+    for name, value in (("q_start", i32(4)), ("kv_len", i32(3)), ("page_table", i32(3, 8)), ("max_q", 3), ("max_kv", 9)):
+        with pytest.raises(AttributeError):
+            setattr(batch, name, value)
+    t = batch._ref(0, 16)._obj
+    assert batch.kv_len is kept and t.kv_len == kept.data_ptr() and (t.max_q, t.max_kv) == (2, 100)
+
+
+def test_what_a_batch_keeps_is_bounded(nb):
+    batch = nb.KvBatch(i32(4), i32(3), i32(3, 8), 2, 100)
+    for stream in range(1, 1000):
+        t = batch._ref(stream, 16)._obj
+        assert t.stream == stream
+    assert len(batch._structs) <= 64
