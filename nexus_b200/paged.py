@@ -213,8 +213,8 @@ class PagedKvCache:
         position i when j > i - window or j < sinks.  `scale` (default
         1/sqrt(head_dim)) is positive; `out` may be q itself.  Rows outside
         every sequence are left as they were (undefined without `out`)."""
-        if window < 0 or sinks < 0:
-            raise _invalid("window and sinks must not be negative")
+        if not (0 <= window < 1 << 31 and 0 <= sinks < 1 << 31):  # (the call would see their low 32 bits)
+            raise _invalid("window and sinks must be in [0, 2^31)")
         if scale is not None and not scale > 1e-45:  # 0 in f32 would ask for the default
             raise _invalid("scale must be positive")
         if out is None:

@@ -71,3 +71,12 @@ def test_what_a_batch_keeps_is_bounded(nb):
         t = batch._ref(stream, 16)._obj
         assert t.stream == stream
     assert len(batch._structs) <= 64
+
+
+@pytest.mark.parametrize("value", [-1, 2 ** 31, 2 ** 32, 2 ** 32 + 5])
+@pytest.mark.parametrize("name", ["window", "sinks"])
+def test_window_and_sinks_beyond_32_bits_are_refused(nb, name, value):
+    """2^32 is not a window of 0, which would see the whole context."""
+    c = nb.PagedKvCache.__new__(nb.PagedKvCache)
+    with pytest.raises(nb.NexusError, match="window and sinks"):
+        c.attention(None, None, **{name: value})
