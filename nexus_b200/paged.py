@@ -14,8 +14,10 @@ written, read back and attended in one call each.
 
 Calls run on torch's current stream of the backend's device, return without
 waiting and may be captured into a CUDA graph (the batch's device tensors are
-read when the graph runs).  ``cache.status()`` waits and raises ``NexusError``
-for what only the device can see, such as a page id beyond the pool.
+read when the graph runs).  They are for serving: rows that require a gradient
+are refused while torch records one.  ``cache.status()`` waits and raises
+``NexusError`` for what only the device can see, such as a page id beyond the
+pool.
 """
 from __future__ import annotations
 
@@ -34,6 +36,10 @@ _raw_stream = torch._C._cuda_getCurrentRawStream  # torch.cuda.current_stream().
 
 def _invalid(msg: str) -> L.NexusError:
     return L.NexusError(L.NEXUS_E_INVALID, msg)
+
+
+def _no_backward(what: str) -> L.NexusError:
+    return _invalid(f"{what} has no backward pass: call it under torch.no_grad(), or detach what requires a gradient")
 
 
 def _on(t: torch.Tensor, device: torch.device, what: str) -> None:
@@ -183,6 +189,8 @@ class PagedKvCache:
 
     def append(self, batch: KvBatch, k: torch.Tensor, v: torch.Tensor) -> None:
         """Quantise the batch's rows of k and v ([rows, kv_heads, head_dim]) into their slots."""
+        if (k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
+            raise _no_backward("append")
         bt, rk, rv = self._batch(batch), self._rows(k, "k"), self._rows(v, "v")
         rc = self._lib.nexus_cuda_kv_append(self.backend.handle, self._ref, bt, C.byref(rk), C.byref(rv))
         if rc:
@@ -217,6 +225,8 @@ class PagedKvCache:
             raise _invalid("window and sinks must be in [0, 2^31)")
         if scale is not None and not scale > 1e-45:  # 0 in f32 would ask for the default
             raise _invalid("scale must be positive")
+        if q.requires_grad and torch.is_grad_enabled():
+            raise _no_backward("attention")
         if out is None:
             out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
         bt, rq, ro = self._batch(batch), self._rows(q, "q"), self._rows(out, "out")

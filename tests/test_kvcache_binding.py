@@ -80,3 +80,15 @@ def test_window_and_sinks_beyond_32_bits_are_refused(nb, name, value):
     c = nb.PagedKvCache.__new__(nb.PagedKvCache)
     with pytest.raises(nb.NexusError, match="window and sinks"):
         c.attention(None, None, **{name: value})
+
+
+def test_rows_that_require_a_gradient_are_refused(nb):
+    """There is no backward pass; a result without history would drop the gradient silently."""
+    c = nb.PagedKvCache.__new__(nb.PagedKvCache)
+    x = torch.zeros((2, 4, 64), requires_grad=True)
+    for call in (lambda: c.attention(None, x), lambda: c.append(None, x, x.detach()),
+                 lambda: c.append(None, x.detach(), x)):
+        with pytest.raises(nb.NexusError, match="no backward pass"):
+            call()
+        with torch.no_grad(), pytest.raises(AttributeError):  # past the check, on to the (missing) batch
+            call()
