@@ -31,7 +31,10 @@ from .engine import CudaBackend
 
 _FORMATS = {torch.float32: L.F32, torch.float16: L.F16, torch.bfloat16: L.BF16}
 _KEPT = 64  # structs and sizes a batch keeps (a long-lived one may meet any number of streams)
-_raw_stream = torch._C._cuda_getCurrentRawStream  # torch.cuda.current_stream().cuda_stream without its object
+# torch.cuda.current_stream(device).cuda_stream; the form without its object is
+# not part of torch's interface, so that a torch without it is served by the other
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
 def _invalid(msg: str) -> L.NexusError:

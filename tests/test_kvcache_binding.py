@@ -92,3 +92,18 @@ def test_rows_that_require_a_gradient_are_refused(nb):
             call()
         with torch.no_grad(), pytest.raises(AttributeError):  # past the check, on to the (missing) batch
             call()
+
+
+def test_the_binding_needs_torchs_public_interface_only():
+    """A torch without the private lookup of the current stream: torch.cuda.current_stream serves."""
+    code = """
+import torch
+from types import SimpleNamespace
+if hasattr(torch._C, "_cuda_getCurrentRawStream"):
+    del torch._C._cuda_getCurrentRawStream
+torch.cuda.current_stream = lambda device: SimpleNamespace(cuda_stream=1234 + device)
+from nexus_b200 import paged
+print(paged._raw_stream(1))
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True)
+    assert r.returncode == 0 and r.stdout == "1235\n", r.stderr
