@@ -787,22 +787,18 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
         const uint32_t *table = p.batch.table + (size_t)b * p.batch.stride;
         const uint32_t mask = (1u << p.cache.shift) - 1u;
         // Lane l < 8: the page of run l (16 tokens) of tile i, ~0 where nothing of it is
-        // read.  (Loaded two tiles ahead; looked at by page_ok.)
+        // read (a table's own ~0 is taken for the one before, as far beyond any pool).
+        // Loaded two tiles ahead; looked at by page_ok.
         auto load_pages = [&](uint32_t i) -> uint32_t {
             if (i >= n || lane >= kTok / 16) return ~0u;
             const uint32_t j = tile_token(i) + 16 * lane;
-            return kv_needed(range, j, j + 16) ? __ldg(table + (j >> p.cache.shift)) : ~0u;
+            return kv_needed(range, j, j + 16) ? min(__ldg(table + (j >> p.cache.shift)), ~1u) : ~0u;
         };
         bool no_page = false;  // lane l < 8: run l of the tile is read and has no page in the pool
-        auto page_ok = [&](uint32_t page, uint32_t i) -> uint32_t {
-            no_page = false;
-            if (page < p.cache.num_pages) return page;
-            if (i < n && lane < kTok / 16) {
-                const uint32_t j = tile_token(i) + 16 * lane;
-                no_page = kv_needed(range, j, j + 16);
-                if (no_page) fault = KV_FAULT_PAGE;
-            }
-            return ~0u;
+        auto page_ok = [&](uint32_t page) -> uint32_t {
+            no_page = page >= p.cache.num_pages && page != ~0u;
+            if (no_page) fault = KV_FAULT_PAGE;
+            return page < p.cache.num_pages ? page : ~0u;
         };
         auto slot_of = [&](uint32_t page, uint32_t j) {
             return (((size_t)page * p.cache.hkv + h) << p.cache.shift) + (j & mask);
@@ -883,7 +879,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
             // power of two on the values' scales and zeros (0: none of them seen so far
             // but zero), the same in both warps, and its reciprocal
             float lift = 0.0f, unit = 1.0f;
-            uint32_t cur = page_ok(next, 0);
+            uint32_t cur = page_ok(next);
             if (n > 0) {
                 load_codes(kbits, kr, p.cache.codes[0], cur, 0);
                 load_scales(cur, 0);
@@ -937,10 +933,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
                         sts1(sl + Slot::ZMAX + 4 * (pw + 2 * t), zm);
                     }
                 }
-                const uint32_t bad = __ballot_sync(0xffffffffu, no_page);
-                if (pt == 0) {
-                    sts1(sl + Slot::UNIT, unit);
-                    sts1(sl + Slot::BAD, __uint_as_float(bad));
+                if (pt == 0) sts1(sl + Slot::UNIT, unit);
+                if (pw == 0) {
+                    const uint32_t bad = __ballot_sync(0xffffffffu, no_page);
+                    if (lane == 0) sts1(sl + Slot::BAD, __uint_as_float(bad));
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
@@ -948,7 +944,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
                     mbar_arrive(&scfull[i % kScaleSlots]);
                     mbar_arrive(&kfull[st]);
                 }
-                cur = page_ok(next, i + 1);
+                cur = page_ok(next);
                 if (i + 1 < n) {
                     load_codes(kbits, kr, p.cache.codes[0], cur, i + 1);
                     load_scales(cur, i + 1);
@@ -959,7 +955,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
         } else {
             const std::integral_constant<int, BV> vbits{};
             uint4 vr[Chunks<D, BV>::N];
-            if (n > 0) load_codes(vbits, vr, p.cache.codes[1], page_ok(next, 0), 0);
+            if (n > 0) load_codes(vbits, vr, p.cache.codes[1], page_ok(next), 0);
             next = load_pages(1);
             for (uint32_t i = 0; i < n; i++) {
                 const uint32_t st = i % ST, ph = (i / ST) & 1;
@@ -969,7 +965,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&vfull[st]);
-                const uint32_t cur = page_ok(next, i + 1);
+                const uint32_t cur = page_ok(next);
                 if (i + 1 < n) load_codes(vbits, vr, p.cache.codes[1], cur, i + 1);
                 next = load_pages(i + 2);
             }
