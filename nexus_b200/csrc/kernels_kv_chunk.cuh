@@ -67,8 +67,18 @@ constexpr int kBlk = 128 * 128;         // 128 rows x 64 f16, swizzled
 // for 2^17 such keys (a 2048-token prompt took 136 us at 4, 140 at 10, 142 at 11, 152 at 12,
 // where the sums of weights near the largest already reach f16's end).
 constexpr float kUp = 4.0f, kUpSplit = 11.0f;
-constexpr float kMaxWeight = 65504.0f;  // and it is moved when a weight would leave f16
+constexpr float kMaxWeight = kvf::kMostF16;  // and it is moved when a weight would leave f16
 constexpr float kMaxProb = kvf::kMaxProb;  // log2 of the largest p where values are zero
+// Scores beyond this are taken relative to the largest when a reference is chosen: base + t
+// then, with t the reference wanted as seen from base, rounded once.  Where that leaves the
+// largest weight more than 2^room above the one wanted, the next number up: for steps of up
+// to 2^5 (scores of 2^29) the weight stays within f16 whatever the values, beyond that for
+// values within 2^15 of the first tile's.
+constexpr float kLargeScore = 4194304.0f;
+__device__ __forceinline__ float reference(float base, float t, float room) {
+    const float m = __fadd_rn(base, t);
+    return t - __fsub_rn(m, base) > room ? __fadd_ru(base, t) : m;
+}
 constexpr int kScaleSlots = 4;
 constexpr int kFlush = kKvFlushTiles;
 
@@ -476,48 +486,62 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
             // what has been summed follows: l, z, the output, and the weights of this
             // tile already written.
             auto new_reference = [&](int q0) {
-                float mx[4], my[4];
-#pragma unroll
-                for (int k = 0; k < 4; k++) mx[k] = my[k] = -INFINITY;
+                float mx[4], my[4], base[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                // (a second time, relative to the largest score, where that is a large one)
 #pragma unroll 1
-                for (int q = q0; q < 4; q++) {
+                for (int pass = 0; pass < 2; pass++) {
 #pragma unroll
-                    for (int hh = 0; hh < 2; hh++) {
-                        uint32_t s[16];
-                        tmem_ld_16x256_x4(scol + hh * kHalf + 32 * q, s);
-                        tmem_wait(s);
+                    for (int k = 0; k < 4; k++) mx[k] = my[k] = -INFINITY;
+#pragma unroll 1
+                    for (int q = q0; q < 4; q++) {
 #pragma unroll
-                        for (int kk = 0; kk < 2; kk++) {
-                            const int k = 2 * hh + kk;
-                            const uint32_t bits = whole ? ~0u : seen(k, 32 * q);
+                        for (int hh = 0; hh < 2; hh++) {
+                            uint32_t s[16];
+                            tmem_ld_16x256_x4(scol + hh * kHalf + 32 * q, s);
+                            tmem_wait(s);
 #pragma unroll
-                            for (int t = 0; t < 4; t++) {
-                                const uint32_t at = slc + 4 * (32 * q + 8 * t);
-                                const f2 lv = lds2(at + Slot::LV);
-                                float e0, e1, v0, v1;
-                                upk(mul2(score(s + 4 * t + 2 * kk, lds2(at + Slot::SK), BK == 4 ? lds2(at + Slot::ZK) : 0, k),
-                                         xs2[k]),
-                                    e0, e1);
-                                upk(lv, v0, v1);
-                                e0 = bits >> (8 * t) & 1 ? e0 : -INFINITY;
-                                e1 = bits >> (8 * t + 1) & 1 ? e1 : -INFINITY;
-                                mx[k] = fmaxf(mx[k], fmaxf(e0, e1));
-                                my[k] = fmaxf(my[k], fmaxf(e0 + v0, e1 + v1));
+                            for (int kk = 0; kk < 2; kk++) {
+                                const int k = 2 * hh + kk;
+                                const uint32_t bits = whole ? ~0u : seen(k, 32 * q);
+#pragma unroll
+                                for (int t = 0; t < 4; t++) {
+                                    const uint32_t at = slc + 4 * (32 * q + 8 * t);
+                                    const f2 lv = lds2(at + Slot::LV);
+                                    float e0, e1, v0, v1;
+                                    upk(mul2(score(s + 4 * t + 2 * kk, lds2(at + Slot::SK), BK == 4 ? lds2(at + Slot::ZK) : 0, k),
+                                             xs2[k]),
+                                        e0, e1);
+                                    upk(lv, v0, v1);
+                                    e0 = bits >> (8 * t) & 1 ? e0 - base[k] : -INFINITY;
+                                    e1 = bits >> (8 * t + 1) & 1 ? e1 - base[k] : -INFINITY;
+                                    mx[k] = fmaxf(mx[k], fmaxf(e0, e1));
+                                    my[k] = fmaxf(my[k], fmaxf(e0 + v0, e1 + v1));
+                                }
                             }
                         }
                     }
+                    bool large = false;
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+#pragma unroll
+                        for (int o = 1; o < 4; o <<= 1) {
+                            mx[k] = fmaxf(mx[k], __shfl_xor_sync(0xffffffffu, mx[k], o));
+                            my[k] = fmaxf(my[k], __shfl_xor_sync(0xffffffffu, my[k], o));
+                        }
+                        large |= fabsf(mx[k]) > kLargeScore && fabsf(mx[k]) < INFINITY;
+                    }
+                    if (pass || !__any_sync(0xffffffffu, large)) break;
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        if (fabsf(mx[k]) > kLargeScore && fabsf(mx[k]) < INFINITY) base[k] = mx[k];
                 }
                 float f[4];
                 bool moved = false;
                 unset = false;
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
-#pragma unroll
-                    for (int o = 1; o < 4; o <<= 1) {
-                        mx[k] = fmaxf(mx[k], __shfl_xor_sync(0xffffffffu, mx[k], o));
-                        my[k] = fmaxf(my[k], __shfl_xor_sync(0xffffffffu, my[k], o));
-                    }
-                    const float next = fmaxf(ref[k], fmaxf(ceilf(my[k]) - (SPLIT ? kUpSplit : kUp), ceilf(mx[k]) - kMaxProb));
+                    const float want = fmaxf(ceilf(my[k]) - (SPLIT ? kUpSplit : kUp), ceilf(mx[k]) - kMaxProb);
+                    const float next = fmaxf(ref[k], reference(base[k], want, SPLIT ? 4.0f : 11.0f));
                     f[k] = 1.0f;
                     if (next != ref[k]) {
                         const kvf::Pow2 fl(ref[k], next);

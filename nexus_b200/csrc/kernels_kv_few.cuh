@@ -16,10 +16,9 @@
 // of two, and whatever the scale of the values the weights stay in f16's range
 // with their 11 bits down to 2^-23 of the largest.  Where the values are zero
 // only p bounds m (2^96 at most, and 2^31 of those stay in f32).  p makes up for
-// the magnitude of the values, which later tiles may change at will: for scales
-// and zeros from 2^-86 to beyond 2^100.  Where the first tile that is not all
-// zero has nothing above 2^-80, or something above 2^40, scales and zeros are
-// multiplied by a power of two first (value_lift).
+// the magnitude of the values, which later tiles may change at will: over 2^86
+// down and 2^100 up from those of the first tile that is not all zero, which a
+// power of two brings near one (value_lift).
 //
 // Bound: HBM, the visible codes and scales once (264 bytes a token and head at
 // D = 128 and 8 bits, 144 at 4).  Layout:
@@ -53,6 +52,7 @@ constexpr int kStages = 3;
 // slots used)
 constexpr float kUp = 10.0f;         // log2 of the largest weight under a new reference
 constexpr float kLimit = 32768.0f;   // largest weight any reference stays for
+constexpr float kMostF16 = 65504.0f;
 constexpr float kMaxProb = 96.0f;    // log2 of the largest p
 // f32 queries: what the second f16 of a weight is multiplied by (at most half a step of the
 // first, 2^3 for one of 2^15, so that it stays in f16).  A weight is then off by 2^-36 at
@@ -170,11 +170,11 @@ __device__ __forceinline__ void lds_words(const uint8_t *p, uint32_t (&w)[N], in
 }
 
 // log2 of what scales and zeros are multiplied by when the largest of the first tile that is
-// not all zero is `mag`.  Down, so that p stays clear of f32's lower end (2^-36 and more for a
-// value near 2^40); up by no more than 2^24, so that later values up to 2^104 stay in f32.
+// not all zero is `mag`: to 2^0 .. 2^9, but up by no more than 2^24, so that later values up
+// to 2^104 stay in f32.
 __device__ __forceinline__ int value_lift(float mag) {
     const int e = (int)((__float_as_uint(mag) >> 23) & 0xffu) - 127;
-    return e > 40 ? 40 - e : e < -80 ? 24 : 0;
+    return e > 8 ? 8 - e : min(24, max(0, -e));
 }
 // ---- distributed shared memory of a cluster ----
 __device__ __forceinline__ void cluster_sync() {
@@ -490,7 +490,7 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? (SPLIT ? 3 : 4) : 2) k_
             };
             uint32_t pf[NR][NS][2];
             // Weights against the references, first the old ones: true where they hold.
-            auto weigh = [&](auto masked, bool last_try) -> bool {
+            auto weigh = [&](auto masked, float limit) -> bool {
                 constexpr bool MASK = decltype(masked)::value;
                 f2 pp[NR][2], ww[NR][2];
                 float top = 0.0f;
@@ -520,7 +520,7 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? (SPLIT ? 3 : 4) : 2) k_
                         // a weight above 2^15, or p above 2^96
                         top = fmaxf(fmaxf(top, fmaxf(w0, w1)), fmaxf(p0, p1) * 4.1359031e-25f);
                     }
-                if (!last_try && __any_sync(0xffffffffu, top > kLimit)) return false;
+                if (__any_sync(0xffffffffu, top > limit)) return false;
 #pragma unroll
                 for (int nr = 0; nr < NR; nr++) {
                     l[nr] = add2(l[nr], add2(pp[nr][0], pp[nr][1]));
@@ -544,8 +544,9 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? (SPLIT ? 3 : 4) : 2) k_
                 }
                 return true;
             };
-            // References that hold for this tile; the sums so far follow.
-            auto new_reference = [&]() {
+            // References that hold for this tile, or (higher) the whole numbers after the present
+            // ones; the sums so far follow.
+            auto new_reference = [&](bool higher) {
                 unset = false;
 #pragma unroll
                 for (int nr = 0; nr < NR; nr++) {
@@ -567,7 +568,8 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? (SPLIT ? 3 : 4) : 2) k_
                             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
                             my = fmaxf(my, __shfl_xor_sync(0xffffffffu, my, w));
                         }
-                        const float m1 = fmaxf(m[nr][e], fmaxf(ceilf(mx) - kMaxProb, ceilf(my) - kUp));
+                        const float m1 = higher ? __fadd_ru(m[nr][e], 1.0f)
+                                                : fmaxf(m[nr][e], fmaxf(ceilf(mx) - kMaxProb, ceilf(my) - kUp));
                         cm[e] = ch[e] = cg[e] = 1.0f;
                         if (m1 != m[nr][e]) {
                             const Pow2 f(m[nr][e], m1);
@@ -588,14 +590,15 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? (SPLIT ? 3 : 4) : 2) k_
                 }
                 unset = __any_sync(0xffffffffu, unset);
             };
-            bool renew = unset, last_try = false;
+            // After new references weights are at most 2^kUp, but where a step of f32 at x is
+            // several powers of two (scores of 2^25 and more) those are up to two steps off:
+            // then the next ones.  (Weights of infinite scales or scores stay as they are.)
+            int tries = unset ? 1 : 0;
             while (true) {
-                if (renew) {
-                    new_reference();
-                    last_try = true;
-                }
-                if (whole ? weigh(std::false_type{}, last_try) : weigh(std::true_type{}, last_try)) break;
-                renew = true;
+                if (tries > 0) new_reference(tries > 1);
+                const float limit = tries == 0 ? kLimit : tries < 4 ? kMostF16 : INFINITY;
+                if (whole ? weigh(std::false_type{}, limit) : weigh(std::true_type{}, limit)) break;
+                tries++;
             }
             // ---- O^T += V^T P^T: tokens 2c, 2c + 1, 2c + 8, 2c + 9, dims g * D/8 .. ----
             constexpr int VW = T::RV / 32;  // words per token (0: two bytes)

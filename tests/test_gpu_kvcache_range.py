@@ -273,3 +273,39 @@ def test_messages_of_calls_that_fail_at_once(backend, nb):
     for t in threads:
         t.join()
     assert len(known) == 4 and told <= known
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("bits_v", [8, 4])
+@pytest.mark.parametrize("new", [1, 4, 60])
+@pytest.mark.parametrize("power", range(10, 24, 2))
+def test_scores_of_every_magnitude(backend, nb, power, new, bits_v, dtype):
+    """Scores of 2^18 .. 2^31 and values of 2^-20 .. 2^20: where a step of f32 is some powers of two, the
+    reference of a row has only those to choose from.  The key with the largest score takes all (the
+    next one is half of it below), the output is its value."""
+    lens = [(new, 700), (new, 90)]
+    batch, pages, rows = make_batch(nb, lens, 16)
+    cache = nb.PagedKvCache.empty(backend, pages, 2, 64, 16, (8, bits_v))
+    g = gen(84)
+    sign = torch.where(torch.rand(64, generator=g, device=DEV) < 0.5, -1.0, 1.0)
+    q = (sign * (0.5 + torch.rand((rows, 8, 64), generator=g, device=DEV))).to(DTYPES[dtype])
+    w = 2.0 ** -21 if dtype == "f32" else 2.0 ** -11
+    for step in range(4):
+        for size in (-20, -9, -3, 0, 8, 20) if dtype != "f16" else (-9, -3, 0, 8):
+            fill_random(cache, 85)
+            cache.v_scales.mul_(2.0 ** size)
+            for b, at in ((0, 333), (1, 20)):
+                page, slot = int(batch.page_table[b, at // 16]), at % 16
+                cache.k_codes[page, :, slot] = torch.where(sign > 0, 255, 1).to(torch.uint8)
+                cache.k_scales[page, :, slot, 0] *= 2.0
+            out = cache.attention(batch, q, scale=1.19 ** step * 1.41 ** (step % 2) * 2.0 ** power)
+            for b, at in ((0, 333), (1, 20)):
+                page, slot = int(batch.page_table[b, at // 16]), at % 16
+                v, z = R.side(cache.v_codes[page, :, slot], cache.v_scales[page, :, slot], bits_v)
+                want = (v + z).repeat_interleave(4, 0).expand(new, 8, 64)
+                part = (v.abs() + z.abs()).repeat_interleave(4, 0).expand(new, 8, 64)
+                tol = torch.finfo(DTYPES[dtype]).eps / 2 * want.abs() + (w + 2.0 ** -20) * part
+                if dtype == "f16":
+                    tol += 2.0 ** -25  # half of its last step
+                assert bool(((out[b * new:(b + 1) * new].double() - want).abs() <= tol).all()), (step, size)
+    cache.status()
