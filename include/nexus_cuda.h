@@ -471,9 +471,10 @@ int nexus_cuda_attention_noalloc(nexus_cuda_backend *b, const float *q_dev, cons
  *   8 bits: scale = max|x| / 127,         value = scale * (code - 128)
  *   4 bits: scale = (max x - min x) / 15, zero = min x + 8 * scale,
  *           value = zero + scale * (code - 8)
- * (scale and zero rounded to f32, code the nearest integer, ties to even).  A
- * group that holds a NaN or an infinity, or spans more than f32, reads back
- * as NaN. */
+ * (scale and zero rounded to f32, code the nearest integer, ties to even, held
+ * in 1..255 or 0..15).  A group that holds a NaN or an infinity, or spans more
+ * than f32, reads back as NaN.  Scales that a caller writes itself are not
+ * negative. */
 typedef struct {
     uint32_t kv_heads;
     uint32_t head_dim;      /* 32, 64 or 128 */
@@ -495,7 +496,8 @@ typedef struct {
  * page page_table[b * table_stride + t / page_tokens]; entries of pages that
  * hold no token a call reads or writes are not looked at, and a page may be
  * listed for several sequences that read it, but the slot a call writes must
- * be one sequence's.  q_start, kv_len and page_table are device arrays, so a
+ * be one sequence's: two tokens written to one slot by one call leave any
+ * mixture of their codes and scales.  q_start, kv_len and page_table are device arrays, so a
  * captured call follows their contents; max_q and max_kv are host bounds of
  * what they will hold. */
 typedef struct {
@@ -522,7 +524,8 @@ typedef struct {
 } nexus_kv_rows;
 
 /* All calls below are asynchronous on the call's stream, keep nothing between
- * calls and may be captured into a CUDA graph.  Arguments are checked before
+ * calls and may be captured into a CUDA graph (which is not launched after the
+ * backend is destroyed: faults are noted there).  Arguments are checked before
  * anything is launched; what only the device can see (a page id beyond the
  * pool, q_start out of order, lengths beyond max_q, max_kv or the page table)
  * makes the kernels skip the sequence or page and is reported by
@@ -538,8 +541,11 @@ int nexus_cuda_kv_read(nexus_cuda_backend *b, const nexus_kv_cache *cache, const
  * their own tokens already: the query at position i sees key j when j <= i and
  * (window == 0 or j > i - window or j < sinks).  Query head q uses KV head
  * q / (q heads / kv heads); at most 128 query heads per KV head.  scale is
- * at most 2e38, 0 means 1/sqrt(head_dim).  out has q's format and heads; it may
- * be q itself (same data and strides), but must not overlap it otherwise.  The workspace
+ * at most 2e38, 0 means 1/sqrt(head_dim).  Tokens of a page beyond the pool are
+ * left out.  Finite queries, keys below 1e33 and values below 1e31 give finite
+ * outputs as long as scores times log2(e) stay in f32; a row that sees only values
+ * 1e25 times smaller than others of its sequence may lose their low bits.  No
+ * backward pass.  out has q's format and heads; it may be q itself (same data and strides), but must not overlap it otherwise.  The workspace
  * (device, 16-byte aligned, contents free before and after) holds at least
  * nexus_cuda_kv_attention_workspace bytes and belongs to this call until it
  * has run: calls that may overlap need one each. */

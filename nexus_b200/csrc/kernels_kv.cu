@@ -2,7 +2,8 @@
 // reading them back.
 //
 // One group is the D elements of one (token, KV head) of keys or values:
-//   8 bits: scale = fl(max|x| / 127),  code = rne(x / scale) + 128
+//   8 bits: scale = fl(max|x| / 127),  code = rne(x / scale) + 128, the integer held
+//           in -127..127 (a subnormal scale can be rounded down by a third)
 //   4 bits: scale = fl((max - min) / 15), zero = fl(min + 8 * scale),
 //           code = rne((x - zero) / scale) + 8, clamped to 0..15
 // with rne the nearest integer, ties to even, of the exact quotient: the

@@ -5,7 +5,7 @@
 //   x_rj = c_r (sk_j (q_r . kc_j) + zk_j sum(q_r)),  p = 2^(x - ref_r)
 //   o_r  = ( sum_j (p sv_j) vc_j + sum_j p zv_j ) / sum_j p
 // kc, vc integer codes around zero (exact in f16), q as f16 (hi + lo for f32
-// queries), the weights p sv rounded to f16 (hi + lo for f32).  ref is a whole
+// queries), the weights p sv rounded to f16 (hi + lo for f32; why, there).  ref is a whole
 // number chosen so that the largest p * max(sv, |zv|) of the row lies between
 // 2^(kUp-1) (kUpSplit for f32 queries) and f16's end; it moves only when a weight
 // would pass that, and then by an exact power of two (p alone is kept below 2^96
@@ -31,13 +31,16 @@
 // The tensor cores round each sum toward zero, an error that grows with the number
 // of products summed in place (4.5e-5 of the output after 40000 tokens).  For f32
 // queries the output is therefore taken out of tensor memory every kFlush tiles
-// and added, correctly rounded, to sums in the caller's workspace.
+// and added, correctly rounded, to sums in the caller's workspace (8e-7 to 9e-7 of the
+// output at 1000 to 131000 tokens; what is left is the two tiles' own sums).
 // Every wait is bounded (as in kernels_gemm.cuh).
-// Measured (32/8 heads, D = 128, 8 bits, bf16): 4096-token prompt 239 us (575
-// TFLOP/s), 2048 tokens behind 14336 751 us (687 TFLOP/s; 0.41 of the measured bf16
-// peak), 256 behind 16128 126 us.  A key tile takes 5400 cycles for both row tiles: the
-// softmax 3600, dependent latencies of two warps a scheduler (a quarter of the issue
-// slots), then 1800 until the tile's products are back; the tensor pipe needs 2048.
+// Measured (32/8 heads, D = 128, 8 bits, device time): bf16 4096-token prompt 238 us (578
+// TFLOP/s), 2048 tokens behind 14336 744 us (693 TFLOP/s; 0.41 of the measured bf16
+// peak), 256 behind 16128 126 us; f32 2048-token prompt 143 us (241 TFLOP/s, each product
+// twice).  In the bf16 prompt the tensor pipe is active in 28% of the cycles and 43% of the
+// issue slots are used, with 0.6 warps ready a scheduler: a row tile's softmax (dependent
+// latencies of its four warps) and its products follow one another, and only the other row
+// tile's fill the gap.
 #pragma once
 #include <type_traits>
 
@@ -298,7 +301,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
     const uint32_t tmem = tmem_base_s;
 
     if (warp < 8) {
-        // ================= softmax: a thread owns a row =================
+        // ================= softmax: a thread has four rows, a quarter of the columns =================
         set_regs<kRegsSoftmax>();
         const int sub = warp >> 2, wq = warp & 3;
         const uint32_t t_lane = (uint32_t)(32 * wq) << 16;
@@ -736,7 +739,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attn_chunk(KvAttnParams p) {
             const bool valid = in_tile < rows.n;
             const float l = row_x[in_tile], z = row_sum[in_tile];
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            const uint32_t tile_id = (b * p.cache.hkv + h) * p.row_tiles + rt;
             const bool split_part = p.nsplit > 1;
             // Rows go through the warp's quarter of its Q tile (every product has completed),
             // 16-byte chunks XORed with the row, so that a row leaves in whole lines: in the

@@ -10,7 +10,10 @@
 // so the two products run on exact small integers in f16 and everything that
 // is not an integer stays in f32.  The rounded factors are q (22 bits as f16
 // hi + lo for f32 queries, 11 bits otherwise: bf16 and f16 are exact) and the
-// weight p sv (f16; hi + lo for f32 queries).  The reference m is a whole
+// weight p sv (f16; hi + lo for f32 queries).  One f16 a weight is what the tensor cores
+// multiply at full rate: each is off by 2^-12 at most, either way, which leaves outputs of
+// 16 bits as far from the 64-bit ones as f32 weights do (1.7e-3 in bf16, 2.1e-4 in f16,
+// of either).  The reference m is a whole
 // number that puts the largest p * max(sv, |zv|) of the row at 2^9 .. 2^10 when
 // it is set and is set anew when that passes 2^15: rescaling is by exact powers
 // of two, and whatever the scale of the values the weights stay in f16's range
@@ -33,10 +36,11 @@
 //    is resident at once, are a cluster, which joins them through distributed shared
 //    memory (parts beyond a sequence's end leave at once); otherwise they go to the
 //    workspace and k_kv_merge joins them.  Either way in order.
-// Measured: 64 sequences of 1024 to 8192 tokens, 32/8 heads, bf16: 114 us at 4 bits
-// (3.0 TB/s; bound by the instructions that unpack and the latencies of a tile's
-// chain), 133 us at 8 bits (4.7 TB/s); one of 131071 tokens, 64/8 heads, f16, 8 bits:
-// 59 us with its join (4.7 TB/s).
+// Measured (device time): 64 sequences of 1024 to 8192 tokens, 32/8 heads: bf16 115 us at
+// 4 bits (3.0 TB/s; 65% of the issue slots, for the unpacking and a tile's chain), 123 us
+// at 8 bits (5.1 TB/s), f32 152 us at 8 bits (4.1 TB/s); 16 sequences of 1000 to 6000
+// tokens with four new ones each, 8 bits, bf16: 56 us; one of 131071 tokens, 64/8 heads,
+// f16, 8 bits: 58 us with its join (4.7 TB/s).
 #pragma once
 #include <type_traits>
 
@@ -48,8 +52,7 @@ namespace kvf {
 constexpr int kWarps = kKvFewWarps;
 constexpr int kStages = 3;
 // Four CTAs an SM (16 warps) for 16-bit queries of up to 8 rows: the loop is a chain
-// of short latencies, and the warps are what hides them (12 warps: 57% of the issue
-// slots used)
+// of short latencies, and the warps are what hides them
 constexpr float kUp = 10.0f;         // log2 of the largest weight under a new reference
 constexpr float kLimit = 32768.0f;   // largest weight any reference stays for
 constexpr float kMostF16 = 65504.0f;
