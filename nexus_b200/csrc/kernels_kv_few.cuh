@@ -596,12 +596,16 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? (SPLIT ? 3 : 4) : 2) k_
             // After new references weights are at most 2^kUp, but where a step of f32 at x is
             // several powers of two (scores of 2^25 and more) those are up to two steps off:
             // then the next ones.  (Weights of infinite scales or scores stay as they are.)
-            int tries = unset ? 1 : 0;
+            bool renew = unset;
+            float limit = kLimit;
+            int tries = 0;
             while (true) {
-                if (tries > 0) new_reference(tries > 1);
-                const float limit = tries == 0 ? kLimit : tries < 4 ? kMostF16 : INFINITY;
+                if (renew) {
+                    new_reference(tries > 0);
+                    limit = ++tries < 4 ? kMostF16 : INFINITY;
+                }
                 if (whole ? weigh(std::false_type{}, limit) : weigh(std::true_type{}, limit)) break;
-                tries++;
+                renew = true;
             }
             // ---- O^T += V^T P^T: tokens 2c, 2c + 1, 2c + 8, 2c + 9, dims g * D/8 .. ----
             constexpr int VW = T::RV / 32;  // words per token (0: two bytes)
